@@ -17,6 +17,7 @@
 #include "../../include/flashtrie_b200.h"
 #include "device/cuda_util.hpp"
 #include "device/device_trie.hpp"
+#include "device/head_ops.hpp"
 #include "engine.hpp"
 #include "host/marisa_image.hpp"
 
@@ -90,6 +91,10 @@ int guarded(F &&f) {
 void require_trie(const ft_trie *t) {
   if (t == nullptr) ftb::fail(ftb::ErrorKind::kNull, "MARISA_NULL_ERROR: trie handle is NULL");
   if (!t->image) ftb::fail(ftb::ErrorKind::kState, "MARISA_STATE_ERROR: trie_.get() == NULL");
+}
+
+void require_args(const void *a, const void *b = "") {
+  if (!a || !b) ftb::fail(ftb::ErrorKind::kNull, "MARISA_NULL_ERROR: NULL argument");
 }
 
 void drop_device(ft_trie *t) {
@@ -281,6 +286,72 @@ int ft_trie_device_status(ft_trie *trie, uint32_t *status) {
     if (!status) ftb::fail(ftb::ErrorKind::kNull, "MARISA_NULL_ERROR: status is NULL");
     if (!trie->engine) ftb::fail(ftb::ErrorKind::kState, "MARISA_STATE_ERROR: no GPU workspace");
     *status = trie->engine->read_status();
+  });
+}
+
+int ft_adapter_logits_workspace(const ft_adapter_args *args, uint64_t *bytes) {
+  return guarded([&] {
+    require_args(args, bytes);
+    *bytes = ftb::adapter_logits_workspace(*args);
+  });
+}
+
+int ft_adapter_logits_device(const ft_adapter_args *args, void *workspace, uint64_t workspace_bytes, void *stream) {
+  return guarded([&] {
+    require_args(args);
+    ftb::adapter_logits_device(*args, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int ft_propose_workspace(const ft_propose_args *args, uint64_t *bytes) {
+  return guarded([&] {
+    require_args(args, bytes);
+    *bytes = ftb::propose_workspace(*args);
+  });
+}
+
+int ft_propose_device(const ft_propose_args *args, void *workspace, uint64_t workspace_bytes, void *stream) {
+  return guarded([&] {
+    require_args(args);
+    ftb::propose_device(*args, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int ft_sequence_logp_workspace(const ft_sequence_args *args, uint64_t *bytes) {
+  return guarded([&] {
+    require_args(args, bytes);
+    *bytes = ftb::sequence_logp_workspace(*args);
+  });
+}
+
+int ft_sequence_logp_device(const ft_sequence_args *args, void *workspace, uint64_t workspace_bytes, void *stream) {
+  return guarded([&] {
+    require_args(args);
+    ftb::sequence_logp_device(*args, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int ft_sequence_grad_device(const ft_sequence_args *args, const float *grad, const float *factor, const float *upstream,
+                            void *workspace, uint64_t workspace_bytes, void *stream) {
+  return guarded([&] {
+    require_args(args);
+    ftb::sequence_grad_device(*args, grad, factor, upstream, workspace, workspace_bytes,
+                              static_cast<cudaStream_t>(stream));
+  });
+}
+
+int ft_preference_loss_workspace(const ft_sequence_args *args, uint32_t pairs, uint64_t *bytes) {
+  return guarded([&] {
+    require_args(args, bytes);
+    *bytes = ftb::preference_workspace(*args, pairs);
+  });
+}
+
+int ft_preference_loss_device(const ft_sequence_args *args, const ft_preference_args *pref, void *workspace,
+                              uint64_t workspace_bytes, void *stream) {
+  return guarded([&] {
+    require_args(args, pref);
+    ftb::preference_loss_device(*args, *pref, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
   });
 }
 

@@ -1,0 +1,164 @@
+// Streaming over rows of logits (f32, bf16 or f16, any alignment) and the
+// running maximum and sum of a softmax.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace ftb {
+
+constexpr float kNegInf = -__builtin_huge_valf();
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+// One rounding to nearest.
+__device__ __forceinline__ void from_f32(float v, float &o) { o = v; }
+__device__ __forceinline__ void from_f32(float v, __nv_bfloat16 &o) { o = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void from_f32(float v, __half &o) { o = __float2half_rn(v); }
+
+// 2^x; the argument is a difference to a maximum, at most a rounding above 0.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A row's elements lie in 16-byte vectors counted from the aligned address at
+// or below its first element; vector i holds elements [i*N - head, i*N - head + N).
+template <typename T>
+struct RowVecs {
+  static constexpr int N = 16 / (int)sizeof(T);
+  const T *row;
+  int64_t len;
+  int head;
+  __device__ RowVecs(const T *r, int64_t n) : row(r), len(n), head((int)((reinterpret_cast<uintptr_t>(r) & 15) / sizeof(T))) {}
+  __device__ int64_t count() const { return (head + len + N - 1) / N; }
+  // First element of vector i (may lie before the row for i = 0).
+  __device__ int64_t first(int64_t i) const { return i * N - head; }
+  __device__ bool whole(int64_t i) const { return first(i) >= 0 && first(i) + N <= len; }
+  __device__ uint4 load_whole(int64_t i) const { return __ldg(reinterpret_cast<const uint4 *>(row + first(i))); }
+  // The vector's values; elements outside the row read as -inf, and none of
+  // them is touched in memory.
+  __device__ void load_edge(int64_t i, float (&v)[N]) const {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const int64_t at = first(i) + e;
+      v[e] = (at >= 0 && at < len) ? to_f32(row[at]) : kNegInf;
+    }
+  }
+};
+
+__device__ __forceinline__ void unpack(uint4 q, float (&v)[4], const float *) {
+  v[0] = __uint_as_float(q.x), v[1] = __uint_as_float(q.y), v[2] = __uint_as_float(q.z), v[3] = __uint_as_float(q.w);
+}
+__device__ __forceinline__ void unpack(uint4 q, float (&v)[8], const __nv_bfloat16 *) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+  }
+}
+__device__ __forceinline__ void unpack(uint4 q, float (&v)[8], const __half *) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+
+// Running (maximum, sum of exp(x - maximum)).  A NaN or +inf among the values
+// leaves the sum NaN; nothing but -inf leaves (-inf, 0).
+struct SoftSum {
+  float m, z;
+  __device__ static SoftSum none() { return {kNegInf, 0.0f}; }
+  __device__ bool valid() const { return z > 0.0f && z < -kNegInf; }  // false for NaN too
+};
+
+__device__ __forceinline__ float exp_from(float x, float m) {
+  return exp2_fast((x - (m == kNegInf ? 0.0f : m)) * kLog2e);
+}
+
+template <int N>
+__device__ __forceinline__ void soft_add(SoftSum &s, const float (&v)[N]) {
+  float top = v[0];
+#pragma unroll
+  for (int e = 1; e < N; ++e) top = fmaxf(top, v[e]);
+  if (top > s.m) {
+    s.z *= exp_from(s.m, top);
+    s.m = top;
+  }
+  const float base = s.m == kNegInf ? 0.0f : s.m;
+  float a = 0.0f;
+#pragma unroll
+  for (int e = 0; e < N; ++e) a += exp2_fast((v[e] - base) * kLog2e);
+  s.z += a;
+}
+
+__device__ __forceinline__ SoftSum soft_join(SoftSum a, SoftSum b) {
+  SoftSum r;
+  r.m = fmaxf(a.m, b.m);
+  r.z = a.z * exp_from(a.m, r.m) + b.z * exp_from(b.m, r.m);
+  return r;
+}
+
+// Joins the block's partial sums in a fixed order; thread 0 has the result.
+template <int THREADS>
+__device__ SoftSum soft_join_block(SoftSum s, SoftSum *smem /* [THREADS / 32] */) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) {
+    SoftSum o{__shfl_xor_sync(~0u, s.m, d), __shfl_xor_sync(~0u, s.z, d)};
+    s = soft_join(s, o);
+  }
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    for (int w = 1; w < THREADS / 32; ++w) s = soft_join(s, smem[w]);
+  return s;
+}
+
+// Adds the vectors [v0, v1) of a row to this thread's sum, U vectors of each
+// thread in flight at a time.
+template <typename T, int THREADS, int U>
+__device__ __forceinline__ void soft_stream(const RowVecs<T> &r, int64_t v0, int64_t v1, SoftSum &s) {
+  constexpr int N = RowVecs<T>::N;
+  int64_t i = v0 + threadIdx.x;
+  for (; i + (U - 1) * THREADS < v1; i += U * THREADS) {
+    if (r.whole(i) && r.whole(i + (U - 1) * THREADS)) {
+      uint4 q[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) q[u] = r.load_whole(i + u * THREADS);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float v[N];
+        unpack(q[u], v, (const T *)nullptr);
+        soft_add(s, v);
+      }
+    } else {
+#pragma unroll 1
+      for (int u = 0; u < U; ++u) {
+        float v[N];
+        r.load_edge(i + u * THREADS, v);
+        soft_add(s, v);
+      }
+    }
+  }
+  for (; i < v1; i += THREADS) {
+    float v[N];
+    if (r.whole(i))
+      unpack(r.load_whole(i), v, (const T *)nullptr);
+    else
+      r.load_edge(i, v);
+    soft_add(s, v);
+  }
+}
+
+}  // namespace ftb

@@ -24,11 +24,23 @@ caller (an event, or stream.wait_stream), and the outputs are allocated on
 [n, cap] ascending; lengths int32 [n, cap]; tokens int32 [n, cap, L], beam j
 of request i in tokens[i, j, :lengths[i, j]]; with key_ids=True also key ids
 int32 [n, cap] (LoudsTrie::lookup's id of each result, read as unsigned).
+
+The steps between a model and the search, on the same tensors and with the
+same stream rules:
+
+    logits = fd.adapter_logits(hidden, weight, adapter_ids, lora_a, lora_b)  # [n, L, V]
+    topk_id, topk_logp = fd.propose(logits, 1000)            # the search's proposals
+    out = fd.bs_tbs_hidden(trie, beams, hidden, weight, 1000, -10.0, -40.0, 5.0, False)  # both, and the search
+    count, lpn, lens, toks = out
+    ref = fd.sequence_logp(ref_logits, toks, lens)           # scores of the results, differentiable
+    loss, margin = fd.preference_loss(logits, toks, lens, ref, chosen, rejected)  # differentiable
 """
 import ctypes
+import math
 import os
 
 import torch
+from torch.autograd.function import once_differentiable
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 _LIB = None
@@ -45,6 +57,34 @@ class _Batch(ctypes.Structure):
                 ("out_capacity", ctypes.c_uint32)] + [(f, ctypes.c_void_p) for f in
                                                       ("beams", "topk_id", "topk_logp", "out_count", "out_lpn",
                                                        "out_len", "out_tok", "out_key")]
+
+
+class _AdapterArgs(ctypes.Structure):
+    _fields_ = [(f, ctypes.c_uint32) for f in ("n", "num_outpos", "vocab", "dim", "rank", "num_adapters")] + \
+        [("dtype", ctypes.c_int32), ("out_dtype", ctypes.c_int32)] + \
+        [(f, ctypes.c_void_p) for f in ("hidden", "weight", "adapter_ids", "lora_a", "lora_b", "scale", "out")]
+
+
+class _ProposeArgs(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_uint64), ("vocab", ctypes.c_uint32), ("topk", ctypes.c_uint32),
+                ("dtype", ctypes.c_int32), ("order", ctypes.c_int32)] + \
+        [(f, ctypes.c_void_p) for f in ("logits", "topk_id", "topk_logp")]
+
+
+class _SequenceArgs(ctypes.Structure):
+    _fields_ = [(f, ctypes.c_uint32) for f in ("n", "num_outpos", "vocab", "candidates")] + \
+        [("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)] + \
+        [(f, ctypes.c_void_p) for f in ("logits", "tokens", "lengths", "stats", "logp", "grad_logits")]
+
+
+class _PreferenceArgs(ctypes.Structure):
+    _fields_ = [("pairs", ctypes.c_uint32), ("mean", ctypes.c_int32), ("beta", ctypes.c_float),
+                ("label_smoothing", ctypes.c_float)] + \
+        [(f, ctypes.c_void_p) for f in ("ref_logp", "chosen", "rejected", "margin", "loss", "grad", "factor")]
+
+
+# FT_DTYPE_* of include/flashtrie_b200.h.
+_DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 def _lib():
@@ -64,6 +104,16 @@ def _lib():
         lib.ft_trie_device_status.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_uint32)]
         lib.ft_trie_device_status.restype = ctypes.c_int
         lib.ft_last_error.restype = ctypes.c_char_p
+        u64p, vp, u32, u64 = ctypes.POINTER(ctypes.c_uint64), ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint64
+        for name, args in (("adapter_logits", _AdapterArgs), ("propose", _ProposeArgs),
+                           ("sequence_logp", _SequenceArgs)):
+            size, call = getattr(lib, "ft_%s_workspace" % name), getattr(lib, "ft_%s_device" % name)
+            size.argtypes = [ctypes.POINTER(args), u64p]
+            call.argtypes = [ctypes.POINTER(args), vp, u64, vp]
+        lib.ft_sequence_grad_device.argtypes = [ctypes.POINTER(_SequenceArgs), vp, vp, vp, vp, u64, vp]
+        lib.ft_preference_loss_workspace.argtypes = [ctypes.POINTER(_SequenceArgs), u32, u64p]
+        lib.ft_preference_loss_device.argtypes = [ctypes.POINTER(_SequenceArgs), ctypes.POINTER(_PreferenceArgs), vp,
+                                                  u64, vp]
         _LIB = lib
     return _LIB
 
@@ -218,3 +268,290 @@ def to_lists(out):
         if len(host) > 4:
             keys.append(host[4][i, :c].numpy().view("uint32").tolist())
     return (sents, lpns, keys) if len(host) > 4 else (sents, lpns)
+
+
+def _want_floating(t, name, ndim, device, dtypes):
+    """_want for a tensor of one of several floating types."""
+    dtype = t.dtype if isinstance(t, torch.Tensor) and t.dtype in dtypes else dtypes[0]
+    _want(t, name, dtype, ndim, device)
+
+
+def _no_gradient(what, **tensors):
+    if torch.is_grad_enabled():
+        for name, t in tensors.items():
+            if t is not None and t.requires_grad:
+                raise ValueError("%s has no gradient: detach %s or call it under torch.no_grad()" % (what, name))
+
+
+def _workspace(size_call, device):
+    """The workspace a call asks for, on the current stream."""
+    need = ctypes.c_uint64(0)
+    _check(size_call(ctypes.byref(need)))
+    return torch.empty(need.value, dtype=torch.uint8, device=device)
+
+
+def _raw_stream(device):
+    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def _on(stream, device):
+    return torch.cuda.stream(torch.cuda.current_stream(device) if stream is None else stream)
+
+
+def adapter_logits(hidden, weight, adapter_ids=None, lora_a=None, lora_b=None, scale=None, out_dtype=None, stream=None):
+    """Logits of n requests over the vocabulary, each request with a low-rank
+    adapter of its own beside the shared projection (C ABI
+    ft_adapter_logits_device):
+
+        out[i] = hidden[i] @ weight.T + scale[a] * (hidden[i] @ lora_a[a].T) @ lora_b[a].T,  a = adapter_ids[i]
+
+    hidden: bfloat16 or float16 [n, L, D]; weight [V, D], lora_a [G, r, D]
+    and lora_b [G, V, r] of the same type; adapter_ids int32 [n]; scale
+    float32 [G] (default 1).  D and r are multiples of 8, r <= 256.  An id of
+    -1 takes the shared projection alone; any other id outside [0, G) makes
+    that request's logits NaN.  Without adapter_ids there are no adapters.
+    Products are summed in 32 bits and rounded once.  Returns [n, L, V] of
+    out_dtype (hidden's type, the default, or float32).  For serving: it has
+    no gradient."""
+    _want_floating(hidden, "hidden", 3, None, (torch.bfloat16, torch.float16))
+    dev, dt = hidden.device, hidden.dtype
+    _want(weight, "weight", dt, 2, dev)
+    n, L, D = hidden.shape
+    V = weight.shape[0]
+    if weight.shape[1] != D:
+        raise ValueError("weight must be [V, D] with D = %d, hidden's" % D)
+    out_dtype = dt if out_dtype is None else out_dtype
+    if out_dtype not in (dt, torch.float32):
+        raise ValueError("out_dtype must be hidden's type or torch.float32")
+    G = r = 0
+    if adapter_ids is None:
+        if lora_a is not None or lora_b is not None or scale is not None:
+            raise ValueError("lora_a, lora_b and scale need adapter_ids")
+    else:
+        if lora_a is None or lora_b is None:
+            raise ValueError("adapter_ids needs lora_a and lora_b")
+        _want(adapter_ids, "adapter_ids", torch.int32, 1, dev)
+        _want(lora_a, "lora_a", dt, 3, dev)
+        _want(lora_b, "lora_b", dt, 3, dev)
+        G, r = lora_a.shape[:2]
+        if adapter_ids.shape[0] != n or lora_a.shape[2] != D or tuple(lora_b.shape) != (G, V, r) or G == 0:
+            raise ValueError("adapter_ids must be [n], lora_a [G, r, D] and lora_b [G, V, r] with G >= 1")
+        if scale is not None:
+            _want(scale, "scale", torch.float32, 1, dev)
+            if scale.shape[0] != G:
+                raise ValueError("scale must have one value per adapter")
+    _no_gradient("adapter_logits", hidden=hidden, weight=weight, lora_a=lora_a, lora_b=lora_b, scale=scale)
+    if L == 0 or V == 0 or D == 0:
+        raise ValueError("L, V and D must be positive")
+    with torch.cuda.device(dev), _on(stream, dev):
+        out = torch.empty((n, L, V), dtype=out_dtype, device=dev)
+        a = _AdapterArgs(n, L, V, D, r, G, _DTYPE[dt], _DTYPE[out_dtype], hidden.data_ptr(), weight.data_ptr(),
+                         adapter_ids.data_ptr() if G else None, lora_a.data_ptr() if G else None,
+                         lora_b.data_ptr() if G else None, scale.data_ptr() if scale is not None else None,
+                         out.data_ptr())
+        ws = _workspace(lambda size: _lib().ft_adapter_logits_workspace(ctypes.byref(a), size), dev)
+        _check(_lib().ft_adapter_logits_device(ctypes.byref(a), ctypes.c_void_p(ws.data_ptr()), ws.numel(),
+                                               _raw_stream(dev)))
+    return out
+
+
+def propose(logits, k, order="id", stream=None):
+    """The search's proposals from logits (C ABI ft_propose_device): per
+    position the log-softmax over the vocabulary and its k largest entries,
+    equal logits in order of the token id.  logits: float32, bfloat16 or
+    float16 [n, L, V].  Returns (topk_id int32 [n, L, k], topk_logp float32
+    [n, L, k]), what bs_tbs_device takes.
+
+    order: "id" (ascending token ids, which the search reads without sorting)
+    or "logp" (best first).  Logits of -inf are never proposed: a position
+    with fewer than k others ends with (-1, -3.4028235e38), entries that no
+    search step takes, and a position without a distribution (a NaN or +inf
+    among its logits, or -inf alone) holds nothing else.  1 <= k <= 8192; it
+    may exceed V.  The outputs have no gradient."""
+    _want_floating(logits, "logits", 3, None, (torch.float32, torch.bfloat16, torch.float16))
+    dev = logits.device
+    n, L, V = logits.shape
+    k = int(k)
+    if not 1 <= k <= 8192:
+        raise ValueError("k must be in [1, 8192]")
+    if order not in ("id", "logp"):
+        raise ValueError("order must be 'id' or 'logp'")
+    if V == 0:
+        raise ValueError("the vocabulary is empty")
+    _no_gradient("propose", logits=logits)
+    with torch.cuda.device(dev), _on(stream, dev):
+        ids = torch.empty((n, L, k), dtype=torch.int32, device=dev)
+        lps = torch.empty((n, L, k), dtype=torch.float32, device=dev)
+        if n * L:
+            a = _ProposeArgs(n * L, V, k, _DTYPE[logits.dtype], int(order == "logp"), logits.data_ptr(),
+                             ids.data_ptr(), lps.data_ptr())
+            ws = _workspace(lambda size: _lib().ft_propose_workspace(ctypes.byref(a), size), dev)
+            _check(_lib().ft_propose_device(ctypes.byref(a), ctypes.c_void_p(ws.data_ptr()), ws.numel(),
+                                            _raw_stream(dev)))
+    return ids, lps
+
+
+def bs_tbs_hidden(trie, beams, hidden, weight, k, token_logp_threshold, sents_logp_threshold, length_norm, early_exit,
+                  adapter_ids=None, lora_a=None, lora_b=None, scale=None, logits_dtype=torch.float32, capacity=None,
+                  stream=None, check=True, key_ids=False):
+    """bs_tbs_device from a model's hidden states: adapter_logits (in
+    logits_dtype), the k best proposals of each position, and the search, one
+    after the other on `stream`.  hidden [n, L, D] goes with beams [n, L];
+    the other arguments and the outputs are those of the three calls."""
+    _want(beams, "beams", torch.int32, 2, None)
+    _want_floating(hidden, "hidden", 3, beams.device, (torch.bfloat16, torch.float16))
+    if hidden.shape[:2] != beams.shape:
+        raise ValueError("hidden must be [n, L, D] with n, L matching beams")
+    logits = adapter_logits(hidden, weight, adapter_ids, lora_a, lora_b, scale, out_dtype=logits_dtype, stream=stream)
+    topk_id, topk_logp = propose(logits, k, stream=stream)
+    del logits
+    return bs_tbs_device(trie, beams, topk_id, topk_logp, token_logp_threshold, sents_logp_threshold, length_norm,
+                         early_exit, capacity=capacity, stream=stream, check=check, key_ids=key_ids)
+
+
+def _sequence_args(logits, tokens, lengths, stats, logp=None, grad_logits=None):
+    n, L, V = logits.shape
+    return _SequenceArgs(n, L, V, tokens.shape[1], _DTYPE[logits.dtype], 0, logits.data_ptr(), tokens.data_ptr(),
+                         lengths.data_ptr(), stats.data_ptr(), logp.data_ptr() if logp is not None else None,
+                         grad_logits.data_ptr() if grad_logits is not None else None)
+
+
+def _sequence_grad(logits, tokens, lengths, stats, grad, factor, upstream):
+    """Gradient of the logits, on the current stream (autograd runs it on the
+    forward call's)."""
+    dev = logits.device
+    with torch.cuda.device(dev):
+        out = torch.empty_like(logits)
+        if logits.numel() == 0 or tokens.shape[1] == 0:
+            return out.zero_()
+        a = _sequence_args(logits, tokens, lengths, stats, grad_logits=out)
+        ws = _workspace(lambda size: _lib().ft_sequence_logp_workspace(ctypes.byref(a), size), dev)
+        _check(_lib().ft_sequence_grad_device(
+            ctypes.byref(a), ctypes.c_void_p(grad.data_ptr()),
+            ctypes.c_void_p(factor.data_ptr() if factor is not None else None),
+            ctypes.c_void_p(upstream.data_ptr() if upstream is not None else None), ctypes.c_void_p(ws.data_ptr()),
+            ws.numel(), _raw_stream(dev)))
+    return out
+
+
+class _SequenceLogp(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, lengths):
+        n, L, _ = logits.shape
+        dev = logits.device
+        logp = torch.empty(lengths.shape, dtype=torch.float32, device=dev)
+        stats = torch.empty((n, L, 2), dtype=torch.float32, device=dev)
+        if logp.numel():
+            a = _sequence_args(logits, tokens, lengths, stats, logp=logp)
+            ws = _workspace(lambda size: _lib().ft_sequence_logp_workspace(ctypes.byref(a), size), dev)
+            _check(_lib().ft_sequence_logp_device(ctypes.byref(a), ctypes.c_void_p(ws.data_ptr()), ws.numel(),
+                                                  _raw_stream(dev)))
+        ctx.save_for_backward(logits, tokens, lengths, stats)
+        return logp
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        return _sequence_grad(*ctx.saved_tensors, g.to(torch.float32).contiguous(), None, None), None, None
+
+
+class _PreferenceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, lengths, ref_logp, chosen, rejected, beta, label_smoothing, mean):
+        n, L, _ = logits.shape
+        dev, P = logits.device, chosen.shape[1]
+        stats = torch.empty((n, L, 2), dtype=torch.float32, device=dev)
+        margin = torch.empty((n, P), dtype=torch.float32, device=dev)
+        # Two tensors: a caller may change the loss in place before the backward pass.
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        factor = torch.empty((), dtype=torch.float32, device=dev)
+        grad = torch.empty(ref_logp.shape, dtype=torch.float32, device=dev)
+        a = _sequence_args(logits, tokens, lengths, stats)
+        p = _PreferenceArgs(P, int(mean), beta, label_smoothing, ref_logp.data_ptr(), chosen.data_ptr(),
+                            rejected.data_ptr(), margin.data_ptr(), loss.data_ptr(), grad.data_ptr(),
+                            factor.data_ptr())
+        ws = _workspace(lambda size: _lib().ft_preference_loss_workspace(ctypes.byref(a), P, size), dev)
+        _check(_lib().ft_preference_loss_device(ctypes.byref(a), ctypes.byref(p), ctypes.c_void_p(ws.data_ptr()),
+                                                ws.numel(), _raw_stream(dev)))
+        ctx.save_for_backward(logits, tokens, lengths, stats, grad, factor)
+        ctx.mark_non_differentiable(margin)
+        return loss, margin
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, _):
+        *saved, grad, factor = ctx.saved_tensors
+        return (_sequence_grad(*saved, grad, factor, g.to(torch.float32).contiguous()),) + (None,) * 8
+
+
+def _want_candidates(logits, tokens, lengths):
+    _want_floating(logits, "logits", 3, None, (torch.float32, torch.bfloat16, torch.float16))
+    dev = logits.device
+    _want(tokens, "tokens", torch.int32, 3, dev)
+    _want(lengths, "lengths", torch.int32, 2, dev)
+    n, L, V = logits.shape
+    if tokens.shape[0] != n or tokens.shape[2] != L or lengths.shape != tokens.shape[:2]:
+        raise ValueError("tokens must be [n, C, L] and lengths [n, C] with n, L matching logits [n, L, V]")
+    if L == 0 or V == 0:
+        raise ValueError("L and V must be positive")
+    if tokens.shape[1] > 8192:
+        raise ValueError("at most 8192 candidates per request")
+    return dev
+
+
+def sequence_logp(logits, tokens, lengths, stream=None):
+    """Log-probabilities of candidate sequences under their request's logits
+    (C ABI ft_sequence_logp_device), differentiable in the logits:
+
+        logp[i, j] = sum of log_softmax(logits[i, l])[tokens[i, j, l]] over l < lengths[i, j]
+
+    logits: float32, bfloat16 or float16 [n, L, V]; tokens int32 [n, C, L]
+    (read as unsigned) and lengths int32 [n, C], as bs_tbs_device returns
+    them: empty result slots have length 0 and score 0.  Returns float32
+    [n, C], summed in 64 bits.  A length outside [0, L] gives NaN and no
+    gradient.  A token id >= V, and any token of a position whose logits are
+    all -inf, has log-probability -inf.  The gradient is deterministic; the
+    backward pass runs on the forward call's stream."""
+    dev = _want_candidates(logits, tokens, lengths)
+    with torch.cuda.device(dev), _on(stream, dev):
+        return _SequenceLogp.apply(logits, tokens, lengths)
+
+
+def preference_loss(logits, tokens, lengths, ref_logp, chosen, rejected, beta=0.1, label_smoothing=0.0,
+                    reduction="mean", stream=None):
+    """Preference loss on pairs of candidate sequences (C ABI
+    ft_preference_loss_device), differentiable in the logits:
+
+        margin = beta * ((logp[c] - ref_logp[c]) - (logp[r] - ref_logp[r]))
+        loss = (1 - label_smoothing) * softplus(-margin) + label_smoothing * softplus(margin)
+
+    with logp = sequence_logp(logits, tokens, lengths), ref_logp float32
+    [n, C] the scores under a reference (a constant), and chosen, rejected
+    int32 [n, P] the pairs' candidate slots.  A pair with a negative slot is
+    absent; one with a slot >= C makes the loss NaN.  reduction: "mean" over
+    the pairs that are there (0 without any) or "sum".  Returns (loss, a
+    float32 scalar, and margin, float32 [n, P], 0 for absent pairs, without
+    gradient)."""
+    dev = _want_candidates(logits, tokens, lengths)
+    n, C = lengths.shape
+    _want(ref_logp, "ref_logp", torch.float32, 2, dev)
+    _want(chosen, "chosen", torch.int32, 2, dev)
+    _want(rejected, "rejected", torch.int32, 2, dev)
+    if ref_logp.shape != lengths.shape:
+        raise ValueError("ref_logp must be [n, C]")
+    if chosen.shape[0] != n or rejected.shape != chosen.shape:
+        raise ValueError("chosen and rejected must both be [n, P]")
+    if C == 0:
+        raise ValueError("there are no candidates")
+    if ref_logp.requires_grad and torch.is_grad_enabled():
+        raise ValueError("ref_logp is a constant of the loss: detach it")
+    beta, label_smoothing = float(beta), float(label_smoothing)
+    if not math.isfinite(ctypes.c_float(beta).value):
+        raise ValueError("beta must be finite in 32 bits")
+    if not 0.0 <= label_smoothing <= 1.0:
+        raise ValueError("label_smoothing must be in [0, 1]")
+    if reduction not in ("mean", "sum"):
+        raise ValueError("reduction must be 'mean' or 'sum'")
+    with torch.cuda.device(dev), _on(stream, dev):
+        return _PreferenceLoss.apply(logits, tokens, lengths, ref_logp, chosen, rejected, beta, label_smoothing,
+                                     reduction == "mean")

@@ -215,6 +215,143 @@ int ft_trie_device_status(ft_trie *trie, uint32_t *status);
 int ft_tbs_batch_device_noalloc(ft_trie *trie, const ft_device_batch *batch,
                                 const ft_search_params *params, void *stream);
 
+/*
+ * Model-side operators around the search (no counterpart in the reference,
+ * whose callers bring topk_id / topk_logp with them): the vocabulary
+ * projection that gives the logits, the proposals taken from them, and the
+ * scores and preference loss of the sequences that the search found.
+ *
+ * They belong to no trie.  Every pointer is a device pointer on the current
+ * CUDA device, arrays are dense and row-major; `stream` is a cudaStream_t of
+ * that device.  The calls only enqueue and may be captured into a CUDA graph.
+ * They allocate nothing: the caller passes `workspace`, 256-byte aligned, of
+ * at least the bytes the matching *_workspace call reports, which no other
+ * call may use until this one's work has finished.  Its contents need no
+ * initialisation.
+ */
+#define FT_DTYPE_F32 0
+#define FT_DTYPE_BF16 1
+#define FT_DTYPE_F16 2
+
+/*
+ * Logits of n requests with num_outpos positions each:
+ *   out[i][l][v] = sum_d hidden[i][l][d] weight[v][d]
+ *                + scale[a] sum_r (sum_d hidden[i][l][d] lora_a[a][r][d]) lora_b[a][v][r]
+ * with a = adapter_ids[i].  a = -1: the shared projection alone; any other id
+ * outside [0, num_adapters) makes the request's logits NaN.  hidden, weight,
+ * lora_a and lora_b are dtype (bf16 or f16) and start on 16-byte boundaries;
+ * dim and rank are multiples of 8, rank at most 256; out is out_dtype (the
+ * same type, or f32).  num_adapters = 0: adapter_ids, lora_a, lora_b and
+ * scale are not read.  scale may be NULL (1 for every adapter).  At most
+ * 65536 adapters.
+ */
+typedef struct {
+  uint32_t n;
+  uint32_t num_outpos;
+  uint32_t vocab;
+  uint32_t dim;
+  uint32_t rank;
+  uint32_t num_adapters;
+  int32_t dtype;
+  int32_t out_dtype;
+  const void *hidden;          /* [n][num_outpos][dim]            */
+  const void *weight;          /* [vocab][dim]                    */
+  const int32_t *adapter_ids;  /* [n]                             */
+  const void *lora_a;          /* [num_adapters][rank][dim]       */
+  const void *lora_b;          /* [num_adapters][vocab][rank]     */
+  const float *scale;          /* [num_adapters] or NULL          */
+  void *out;                   /* [n][num_outpos][vocab]          */
+} ft_adapter_args;
+
+int ft_adapter_logits_workspace(const ft_adapter_args *args, uint64_t *bytes);
+int ft_adapter_logits_device(const ft_adapter_args *args, void *workspace, uint64_t workspace_bytes, void *stream);
+
+/*
+ * The search's proposals from logits: per row, log-softmax over the
+ * vocabulary and its topk largest entries, equal logits in order of the token
+ * id.  order 0: each row ascending by id (what the search reads without
+ * sorting); 1: by descending log-probability, then id.  Entries with a logit
+ * of -inf are never proposed; a row with fewer than topk others ends with
+ * entries (0xFFFFFFFF, -FLT_MAX), which no search step takes, and so does,
+ * from its start, a row without a distribution (a NaN or +inf among its
+ * logits, or -inf alone).  topk is in [1, 8192].
+ */
+typedef struct {
+  uint64_t rows;        /* n * num_outpos                 */
+  uint32_t vocab;
+  uint32_t topk;
+  int32_t dtype;
+  int32_t order;
+  const void *logits;   /* [rows][vocab]                  */
+  uint32_t *topk_id;    /* [rows][topk]                   */
+  float *topk_logp;     /* [rows][topk]                   */
+} ft_propose_args;
+
+int ft_propose_workspace(const ft_propose_args *args, uint64_t *bytes);
+int ft_propose_device(const ft_propose_args *args, void *workspace, uint64_t workspace_bytes, void *stream);
+
+/*
+ * Scores of candidate sequences under the logits of their request:
+ *   logp[i][j] = sum over l < lengths[i][j] of log softmax(logits[i][l])[tokens[i][j][l]]
+ * tokens and lengths have the layout of the search's results (out_tok,
+ * out_len with out_capacity = candidates).  Length 0 gives 0; a length
+ * outside [0, num_outpos] gives NaN and takes no part in gradients; tokens
+ * behind a length are not read.  A token id >= vocab counts as a logit of
+ * -inf, and so does every token of a position whose logits are all -inf; such
+ * a position has no gradient.  candidates is at most 8192.  `stats` receives
+ * (maximum, sum of exponentials) of every row, which the gradient reads.
+ */
+typedef struct {
+  uint32_t n;
+  uint32_t num_outpos;
+  uint32_t vocab;
+  uint32_t candidates;
+  int32_t dtype;
+  int32_t reserved;
+  const void *logits;       /* [n][num_outpos][vocab]             */
+  const uint32_t *tokens;   /* [n][candidates][num_outpos]        */
+  const int32_t *lengths;   /* [n][candidates]                    */
+  float *stats;             /* [n][num_outpos][2]                 */
+  float *logp;              /* [n][candidates], NULL: not written */
+  void *grad_logits;        /* [n][num_outpos][vocab], gradients  */
+} ft_sequence_args;
+
+int ft_sequence_logp_workspace(const ft_sequence_args *args, uint64_t *bytes);
+int ft_sequence_logp_device(const ft_sequence_args *args, void *workspace, uint64_t workspace_bytes, void *stream);
+/* grad_logits = the gradient of sum_ij w[i][j] logp[i][j], with w = grad
+ * ([n][candidates]), times *factor and *upstream (device scalars, each may be
+ * NULL).  Reads stats as the forward call left it. */
+int ft_sequence_grad_device(const ft_sequence_args *args, const float *grad, const float *factor,
+                            const float *upstream, void *workspace, uint64_t workspace_bytes, void *stream);
+
+/*
+ * Preference loss on pairs of candidates of the same request:
+ *   margin = beta ((logp[c] - ref_logp[c]) - (logp[r] - ref_logp[r]))
+ *   loss   = sum over pairs of (1 - s) softplus(-margin) + s softplus(margin),
+ * s = label_smoothing; with `mean`, divided by the number of pairs (at least
+ * 1).  A pair with a negative index is absent: margin 0, no loss.  One with
+ * an index >= candidates makes its margin and the loss NaN and has no
+ * gradient.  grad receives d loss / d logp before that division and factor
+ * the division, in the form that ft_sequence_grad_device takes.
+ */
+typedef struct {
+  uint32_t pairs;           /* pairs per request                  */
+  int32_t mean;
+  float beta;
+  float label_smoothing;
+  const float *ref_logp;    /* [n][candidates]                    */
+  const int32_t *chosen;    /* [n][pairs]                         */
+  const int32_t *rejected;  /* [n][pairs]                         */
+  float *margin;            /* [n][pairs]                         */
+  float *loss;              /* [1]                                */
+  float *grad;              /* [n][candidates]                    */
+  float *factor;            /* [1]                                */
+} ft_preference_args;
+
+int ft_preference_loss_workspace(const ft_sequence_args *args, uint32_t pairs, uint64_t *bytes);
+int ft_preference_loss_device(const ft_sequence_args *args, const ft_preference_args *pref, void *workspace,
+                              uint64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
