@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(kStatThreads)
         }
       }
 #pragma unroll
-      for (int e = 0; e < N; ++e) v[e] = k * exp2_fast((v[e] - base) * kLog2e);
+      for (int e = 0; e < N; ++e) v[e] = k * exp_below(v[e] - base);
     }
     if (out.whole(i)) {
       *reinterpret_cast<uint4 *>(g + out.first(i)) = pack(v, (const T *)nullptr);
@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(kStatThreads)
   const uint32_t a = lower_bound(t, n, (uint32_t)e0);
   for (uint32_t i = a + threadIdx.x; i < n && t[i] < e1; i += kStatThreads) {
     if (i > 0 && t[i - 1] == t[i]) continue;
-    const float p = zero ? 0.0f : k * exp2_fast((to_f32(in.row[t[i]]) - base) * kLog2e);
+    const float p = zero ? 0.0f : k * exp_below(to_f32(in.row[t[i]]) - base);
     from_f32(tok_w[row * C + i] + p, g[t[i]]);
   }
 }

@@ -4,10 +4,18 @@
 //
 //   logp[v] = x[v] - m - log(sum_u exp(x[u] - m)),  m = max_u x[u]
 //
-// One CTA per row.  The entries are ordered by the 64-bit key (logit as an
-// ordered integer, complement of the id), which no two share, so the k-th
-// largest key separates the proposals from the rest.  It is found by radix
-// selection, 11 bits a pass.
+// The entries are ordered by the 64-bit key (logit as an ordered integer,
+// complement of the id), which no two share, so the k-th largest key separates
+// the proposals from the rest.
+//
+// The logits are read once.  A row is cut into stretches, a CTA each.  A
+// sample spread over the row gives a bound that about 8 + k + 4 sqrt entries
+// in the sample's measure pass; the CTA streams its stretch, adds to the
+// softmax sum and keeps what passes the bound in shared memory.  The CTA that
+// ends last in its row joins the sums, selects the k largest of what all have
+// kept, and sorts them.  The bound is a guess only: a stretch that keeps more
+// than fits is read again with a bound that rises (`careful`), and a row that
+// kept fewer than k is read again by its last CTA without one.
 #include <algorithm>
 #include <string>
 
@@ -19,9 +27,12 @@
 namespace ftb {
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 512;
 constexpr uint32_t kBins = 2048;
+constexpr uint32_t kSample = 8192;  // sampled entries of a row
 constexpr float kFltMax = 3.402823466e+38f;
+
+typedef unsigned long long Key;
 
 // Order-preserving integer of a float; -0 and 0 are the same.
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -31,92 +42,320 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 __device__ __forceinline__ float unordered(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
+__device__ __forceinline__ Key key_of(float x, int64_t id) { return (Key)ordered(x) << 32 | (uint32_t)~(uint32_t)id; }
 
-template <typename T, typename F>
-__device__ __forceinline__ void for_each(const RowVecs<T> &r, F &&f) {
+struct ProposePlan {
+  uint32_t chunks;      // CTAs per row
+  uint32_t cap;         // entries that a CTA can keep
+  uint32_t emit;        // entries that a CTA hands on
+  uint32_t slots;       // power of two >= k
+  uint64_t vecs_chunk;  // 16-byte vectors per stretch
+};
+
+struct Shared {
+  uint32_t hist[kBins];
+  uint32_t scan[kThreads / 32];
+  Key low[kThreads / 32], high[kThreads / 32];
+  SoftSum sums[kThreads / 32];
+  SoftSum sum;
+  uint32_t count, bin, above;
+  bool last;
+};
+
+// The bin, from the top, in which the need-th entry lies, and the number of
+// entries above it; bin kBins if there are fewer.
+__device__ void find_bin(Shared &sh, uint32_t need, uint32_t &bin, uint32_t &above) {
+  constexpr int kPer = kBins / kThreads;
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __syncthreads();
+  uint32_t mine[kPer], sum = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) sum += mine[i] = sh.hist[kBins - 1 - (threadIdx.x * kPer + i)];
+  uint32_t s = sum;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const uint32_t o = __shfl_up_sync(~0u, s, d);
+    if (lane >= (uint32_t)d) s += o;
+  }
+  if (lane == 31) sh.scan[warp] = s;
+  if (threadIdx.x == 0) sh.bin = kBins, sh.above = 0;
+  __syncthreads();
+  uint32_t before = s - sum;
+  for (uint32_t w = 0; w < warp; ++w) before += sh.scan[w];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    if (before < need && before + mine[i] >= need) sh.bin = kBins - 1 - (threadIdx.x * kPer + i), sh.above = before;
+    before += mine[i];
+  }
+  __syncthreads();
+  bin = sh.bin;
+  above = sh.above;
+}
+
+__device__ void clear_bins(Shared &sh) {
+  __syncthreads();
+  for (uint32_t b = threadIdx.x; b < kBins; b += kThreads) sh.hist[b] = 0;
+  __syncthreads();
+}
+
+__device__ void block_range(Shared &sh, Key &low, Key &high) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) {
+    low = min(low, (Key)__shfl_xor_sync(~0u, low, d));
+    high = max(high, (Key)__shfl_xor_sync(~0u, high, d));
+  }
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sh.low[threadIdx.x >> 5] = low, sh.high[threadIdx.x >> 5] = high;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) low = min(low, sh.low[w]), high = max(high, sh.high[w]);
+}
+
+// Keeps the entries of list[0, count) that are not below the returned key: at
+// least the k largest, and at most k + slack.  Radix selection, 11 bits a
+// pass, from the highest bit in which the entries differ.  count >= k.
+__device__ Key keep_largest(Shared &sh, Key *list, uint32_t count, uint32_t k, uint32_t slack) {
+  Key low = ~0ull, high = 0;
+  for (uint32_t i = threadIdx.x; i < count; i += kThreads) low = min(low, list[i]), high = max(high, list[i]);
+  block_range(sh, low, high);
+  uint32_t need = k, sure = 0;
+  for (;;) {
+    const Key span = high - low;
+    const int bits = span ? 64 - __clzll((long long)span) : 0, shift = bits > 11 ? bits - 11 : 0;
+    clear_bins(sh);
+    for (uint32_t i = threadIdx.x; i < count; i += kThreads) {
+      const Key x = list[i];
+      if (x >= low && x <= high) atomicAdd(&sh.hist[(uint32_t)((x - low) >> shift)], 1u);
+    }
+    uint32_t bin, above;
+    find_bin(sh, need, bin, above);
+    const uint32_t in_bin = sh.hist[bin];
+    low += (Key)bin << shift;
+    if (shift == 0 || sure + above + in_bin <= k + slack) break;
+    high = min(high, low + (((Key)1 << shift) - 1));
+    need -= above;
+    sure += above;
+  }
+  // In place: a round's entries are read before any is written, and no write
+  // goes beyond the entries read so far.
+  __syncthreads();
+  if (threadIdx.x == 0) sh.count = 0;
+  for (uint32_t i0 = 0; i0 < count; i0 += kThreads) {
+    const uint32_t i = i0 + threadIdx.x;
+    const Key x = i < count ? list[i] : 0;
+    __syncthreads();
+    if (i < count && x >= low) list[atomicAdd(&sh.count, 1u)] = x;
+  }
+  __syncthreads();
+  return low;
+}
+
+// One stretch with a bound that rises: whenever the next step might not fit,
+// all but the k largest (and a little more) go.  The ids rise, so what equals
+// the bound's logit later on comes after k others.
+template <typename T>
+__device__ void careful(Shared &sh, Key *list, const RowVecs<T> &r, int64_t v0, int64_t v1, uint32_t k, uint32_t cap) {
   constexpr int N = RowVecs<T>::N;
-  const int64_t n = r.count();
-  for (int64_t i = threadIdx.x; i < n; i += kThreads) {
+  float bound = kNegInf;
+  __syncthreads();
+  if (threadIdx.x == 0) sh.count = 0;
+  for (int64_t i0 = v0; i0 < v1; i0 += kThreads) {
+    __syncthreads();
+    const uint32_t count = sh.count;
+    if (count + kThreads * N > cap) bound = unordered((uint32_t)(keep_largest(sh, list, count, k, 256) >> 32));
+    __syncthreads();
+    const int64_t i = i0 + threadIdx.x;
+    if (i < v1) {
+      float v[N];
+      if (r.whole(i))
+        unpack(r.load_whole(i), v, (const T *)nullptr);
+      else
+        r.load_edge(i, v);
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (v[e] > bound) list[atomicAdd(&sh.count, 1u)] = key_of(v[e], r.first(i) + e);
+    }
+  }
+  __syncthreads();
+}
+
+// A bound below the row's k-th largest logit, from a sample of it (warps read
+// stretches of 32 vectors spread evenly over the row).
+template <typename T>
+__device__ float sample_bound(Shared &sh, const RowVecs<T> &r, uint32_t k) {
+  constexpr int N = RowVecs<T>::N, kLoads = kSample / N / kThreads, kSegments = kLoads * kThreads / 32;
+  const int64_t vecs = r.count();
+  uint32_t key[kLoads][N];
+  uint4 q[kLoads];
+  int64_t at[kLoads];
+#pragma unroll
+  for (int u = 0; u < kLoads; ++u) {
+    const int64_t seg = u * (kThreads / 32) + (threadIdx.x >> 5);
+    at[u] = vecs * seg / kSegments + (threadIdx.x & 31);
+    if (r.whole(at[u])) q[u] = r.load_whole(at[u]);
+  }
+  Key low = 0xFFFFFFFFu, high = 0;
+#pragma unroll
+  for (int u = 0; u < kLoads; ++u) {
     float v[N];
-    if (r.whole(i))
-      unpack(r.load_whole(i), v, (const T *)nullptr);
+    if (r.whole(at[u]))
+      unpack(q[u], v, (const T *)nullptr);
     else
-      r.load_edge(i, v);
+      r.load_edge(at[u], v);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      key[u][e] = v[e] > kNegInf ? ordered(v[e]) : 0;
+      if (key[u][e]) low = min(low, (Key)key[u][e]), high = max(high, (Key)key[u][e]);
+    }
+  }
+  block_range(sh, low, high);
+  if (high == 0) return kNegInf;
+  const uint32_t span = (uint32_t)(high - low);
+  const int bits = 32 - __clz((int)span), shift = bits > 11 ? bits - 11 : 0;
+  clear_bins(sh);
+#pragma unroll
+  for (int u = 0; u < kLoads; ++u)
 #pragma unroll
     for (int e = 0; e < N; ++e)
-      if (v[e] > kNegInf) f(((uint64_t)ordered(v[e]) << 32) | (uint32_t)~(uint32_t)(r.first(i) + e), v[e]);
-  }
+      if (key[u][e]) atomicAdd(&sh.hist[(key[u][e] - (uint32_t)low) >> shift], 1u);
+  // The k-th logit is expected at rank k kSample / V of the sample, give or
+  // take its square root; four of them and 8 more are left for safety.
+  const float rank = (float)k * kSample / (float)r.len;
+  uint32_t bin, above;
+  find_bin(sh, (uint32_t)(rank + 4.0f * sqrtf(rank)) + 8, bin, above);
+  if (bin == kBins) return kNegInf;
+  return unordered((uint32_t)low + (bin << shift) - 1);  // the bin's least logit still passes
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
-    propose_kernel(const T *logits, uint32_t vocab, uint32_t k, int order, uint32_t slots, uint32_t *out_id, float *out_lp) {
-  extern __shared__ unsigned long long list[];
-  __shared__ SoftSum sm[kThreads / 32];
-  __shared__ uint32_t hist[kBins];
-  __shared__ uint32_t got, sm_digit, sm_above;
-  __shared__ SoftSum sm_sum;
-  const uint64_t row = blockIdx.x;
+__global__ void __launch_bounds__(kThreads, 2)
+    propose_kernel(const T *logits, uint32_t vocab, uint32_t k, int order, ProposePlan p, SoftSum *part, uint32_t *counts,
+                   uint32_t *tickets, Key *kept, uint32_t *out_id, float *out_lp) {
+  extern __shared__ Key list[];  // [max(cap, slots)]
+  __shared__ Shared sh;
+  constexpr int N = RowVecs<T>::N;
+  const uint64_t row = blockIdx.x / p.chunks;
+  const uint32_t chunk = blockIdx.x % p.chunks;
   const RowVecs<T> r(logits + row * vocab, vocab);
-  SoftSum s = SoftSum::none();
-  soft_stream<T, kThreads, 4>(r, 0, r.count(), s);
-  s = soft_join_block<kThreads>(s, sm);
-  if (threadIdx.x == 0) sm_sum = s, got = 0;
+  const int64_t v0 = (int64_t)(chunk * p.vecs_chunk), v1 = min(v0 + (int64_t)p.vecs_chunk, r.count());
+  if (threadIdx.x == 0) sh.count = 0;
+  const bool sampled = vocab > p.cap;
+  const float bound = sampled ? sample_bound(sh, r, k) : kNegInf;
   __syncthreads();
-  s = sm_sum;
-  if (s.valid()) {
-    // prefix: the bits of the k-th largest key known so far; need: its rank
-    // among the keys that share them.
-    uint64_t prefix = 0;
-    uint32_t need = k;
-    bool all = false;
-    for (int shift = 53; shift > -11 && !all; shift -= 11) {
-      const int sh = shift < 0 ? 0 : shift, bits = shift < 0 ? 11 + shift : 11;
-      const uint64_t above = sh + bits >= 64 ? 0 : ~0ull << (sh + bits);
-      for (uint32_t b = threadIdx.x; b < kBins; b += kThreads) hist[b] = 0;
-      __syncthreads();
-      for_each(r, [&](uint64_t key, float) {
-        if ((key & above) == prefix) atomicAdd(&hist[(uint32_t)(key >> sh) & ((1u << bits) - 1)], 1u);
-      });
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        uint32_t sum = 0;
-        int d = (1 << bits) - 1;
-        for (; d >= 0; --d) {
-          if (sum + hist[d] >= need) break;
-          sum += hist[d];
+  SoftSum s = SoftSum::none();
+  auto take = [&](int64_t i, const float (&v)[N]) {
+    if (soft_add(s, v) > bound) {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (v[e] > bound) {
+          const uint32_t at = atomicAdd(&sh.count, 1u);
+          if (at < p.cap) list[at] = key_of(v[e], r.first(i) + e);
         }
-        sm_digit = (uint32_t)d;
-        sm_above = sum;
-      }
-      __syncthreads();
-      if ((int)sm_digit < 0) {
-        all = true;  // fewer than k entries: all of them
-      } else {
-        prefix |= (uint64_t)sm_digit << sh;
-        need -= sm_above;
-      }
-      __syncthreads();
     }
-    const uint64_t least = all ? 0 : prefix;
-    for_each(r, [&](uint64_t key, float) {
-      if (key >= least) {
-        const uint32_t at = atomicAdd(&got, 1u);
-        const uint32_t id = ~(uint32_t)key, v = (uint32_t)(key >> 32);
-        list[at] = order == 0 ? ((uint64_t)id << 32) | v : ((uint64_t)~v << 32) | id;
+  };
+  {
+    constexpr int U = 4;
+    int64_t i = v0 + threadIdx.x;
+    for (; i + (U - 1) * kThreads < v1; i += U * kThreads) {
+      if (r.whole(i) && r.whole(i + (U - 1) * kThreads)) {
+        uint4 q[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) q[u] = r.load_whole(i + u * kThreads);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          float v[N];
+          unpack(q[u], v, (const T *)nullptr);
+          take(i + u * kThreads, v);
+        }
+      } else {
+#pragma unroll 1
+        for (int u = 0; u < U; ++u) {
+          float v[N];
+          r.load_edge(i + u * kThreads, v);
+          take(i + u * kThreads, v);
+        }
       }
-    });
-    __syncthreads();
+    }
+    for (; i < v1; i += kThreads) {
+      float v[N];
+      if (r.whole(i))
+        unpack(r.load_whole(i), v, (const T *)nullptr);
+      else
+        r.load_edge(i, v);
+      take(i, v);
+    }
   }
-  const uint32_t n = got;
-  for (uint32_t i = n + threadIdx.x; i < slots; i += kThreads) list[i] = ~0ull;
-  for (uint32_t size = 2; size <= slots; size <<= 1)
+  s = soft_join_block<kThreads>(s, sh.sums);  // a barrier: the list is complete
+  uint32_t count = sh.count;
+  if (count > p.cap) {
+    careful(sh, list, r, v0, v1, k, p.cap);
+    count = sh.count;
+  }
+  if (p.chunks > 1) {
+    // Hand the stretch's sum and entries on; the row's last CTA goes on alone.
+    if (count > p.emit) {
+      keep_largest(sh, list, count, k, 256);
+      count = sh.count;
+    }
+    Key *to = kept + (uint64_t)blockIdx.x * p.emit;
+    for (uint32_t i = threadIdx.x; i < count; i += kThreads) to[i] = list[i];
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      part[blockIdx.x] = s;
+      counts[blockIdx.x] = count;
+      __threadfence();
+      sh.last = atomicAdd(&tickets[row], 1u) == p.chunks - 1;
+    }
+    __syncthreads();
+    if (!sh.last) return;
+    __threadfence();
+    if (threadIdx.x == 0) sh.count = 0;
+    s = SoftSum::none();
+    Key least = 0;
+    for (uint32_t c = 0; c < p.chunks; ++c) {
+      const uint64_t from = row * p.chunks + c;
+      const uint32_t have = __ldcg(&counts[from]);
+      s = soft_join(s, SoftSum{__ldcg(&part[from].m), __ldcg(&part[from].z)});
+      __syncthreads();
+      count = sh.count;
+      if (count + have > p.cap) least = keep_largest(sh, list, count, k, 256);
+      __syncthreads();
+      for (uint32_t i = threadIdx.x; i < have; i += kThreads) {
+        const Key x = __ldcg(&kept[from * p.emit + i]);
+        if (x >= least) list[atomicAdd(&sh.count, 1u)] = x;
+      }
+    }
+    __syncthreads();
+    count = sh.count;
+  }
+  if (sampled && bound > kNegInf && count < k) {
+    careful(sh, list, r, 0, r.count(), k, p.cap);
+    count = sh.count;
+  }
+  if (threadIdx.x == 0) sh.sum = s;
+  __syncthreads();
+  s = sh.sum;
+  if (!s.valid()) count = 0;
+  if (count > k) {
+    keep_largest(sh, list, count, k, 0);
+    count = sh.count;
+  }
+  // Ascending by (id) or by (falling logit, id).
+  for (uint32_t i = threadIdx.x; i < p.slots; i += kThreads) {
+    Key x = ~0ull;
+    if (i < count) {
+      const uint32_t id = ~(uint32_t)list[i], v = (uint32_t)(list[i] >> 32);
+      x = order == 0 ? (Key)id << 32 | v : (Key)~v << 32 | id;
+    }
+    list[i] = x;
+  }
+  for (uint32_t size = 2; size <= p.slots; size <<= 1)
     for (uint32_t step = size >> 1; step; step >>= 1) {
       __syncthreads();
-      for (uint32_t i = threadIdx.x; i < slots / 2; i += kThreads) {
+      for (uint32_t i = threadIdx.x; i < p.slots / 2; i += kThreads) {
         const uint32_t a = 2 * i - (i & (step - 1)), b = a + step;
         const bool up = (a & size) == 0;
-        const unsigned long long x = list[a], y = list[b];
+        const Key x = list[a], y = list[b];
         if ((x > y) == up) list[a] = y, list[b] = x;
       }
     }
@@ -125,8 +364,8 @@ __global__ void __launch_bounds__(kThreads)
   for (uint32_t i = threadIdx.x; i < k; i += kThreads) {
     uint32_t id = 0xFFFFFFFFu;
     float lp = -kFltMax;
-    if (i < n) {
-      const unsigned long long e = list[i];
+    if (i < count) {
+      const Key e = list[i];
       id = order == 0 ? (uint32_t)(e >> 32) : (uint32_t)e;
       const uint32_t v = order == 0 ? (uint32_t)e : ~(uint32_t)(e >> 32);
       lp = (unordered(v) - s.m) - logz;
@@ -146,11 +385,42 @@ void check_propose(const ft_propose_args &a) {
   if (a.rows > 0x7FFFFFFF) throw InvalidArgument("propose: too many rows");
 }
 
+uint64_t align256(uint64_t x) { return (x + 255) & ~(uint64_t)255; }
+
+struct Layout {
+  ProposePlan p;
+  uint64_t part, counts, tickets, kept, end;
+};
+
+Layout layout_of(const ft_propose_args &a) {
+  Layout l;
+  ProposePlan &p = l.p;
+  p.slots = 2;
+  while (p.slots < a.topk) p.slots <<= 1;
+  // Room for what passes the sampled bound: a few thousand entries for small
+  // k, about 1.3 k for large (80 KB at k = 1000: two CTAs per SM).
+  p.cap = 8192 + 2 * a.topk;
+  p.emit = a.topk + 4096;  // cap - emit >= topk: a list that lacks room for another has topk entries
+  const uint64_t vecs = ((uint64_t)a.vocab * (a.dtype == FT_DTYPE_F32 ? 4 : 2) + 15) / 16 + 1;
+  const uint64_t slots = 148 * 2;
+  uint64_t chunks = a.rows ? (a.rows >= slots ? 1 : slots / a.rows) : 1;
+  chunks = std::max<uint64_t>(1, std::min<uint64_t>({chunks, (vecs + 2047) / 2048, 64}));
+  p.vecs_chunk = (vecs + chunks - 1) / chunks;
+  p.chunks = (uint32_t)((vecs + p.vecs_chunk - 1) / p.vecs_chunk);
+  const uint64_t ctas = p.chunks > 1 ? a.rows * p.chunks : 0;
+  l.part = 0;
+  l.counts = align256(sizeof(SoftSum) * ctas);
+  l.tickets = l.counts + align256(4 * ctas);
+  l.kept = l.tickets + align256(p.chunks > 1 ? 4 * a.rows : 0);
+  l.end = l.kept + align256(8 * ctas * p.emit);
+  return l;
+}
+
 }  // namespace
 
 uint64_t propose_workspace(const ft_propose_args &a) {
   check_propose(a);
-  return 0;
+  return layout_of(a).end;
 }
 
 void propose_device(const ft_propose_args &a, void *ws, uint64_t ws_bytes, cudaStream_t stream) {
@@ -160,15 +430,19 @@ void propose_device(const ft_propose_args &a, void *ws, uint64_t ws_bytes, cudaS
     fail(ErrorKind::kNull, "MARISA_NULL_ERROR: propose: logits, topk_id or topk_logp is NULL");
   if (reinterpret_cast<uintptr_t>(a.logits) % (a.dtype == FT_DTYPE_F32 ? 4 : 2))
     throw InvalidArgument("propose: logits is not aligned to its elements");
-  uint32_t slots = 2;
-  while (slots < a.topk) slots <<= 1;
-  const size_t smem = 8ull * slots;
+  const Layout l = layout_of(a);
+  if (ws_bytes < l.end || (l.end && (!ws || (reinterpret_cast<uintptr_t>(ws) & 255))))
+    throw InvalidArgument("propose: needs a 256-byte aligned workspace of " + std::to_string(l.end) + " bytes");
+  uint8_t *w = static_cast<uint8_t *>(ws);
+  if (l.p.chunks > 1) CUDA_TRY(cudaMemsetAsync(w + l.tickets, 0, 4 * a.rows, stream));
+  const size_t smem = 8ull * std::max(l.p.cap, l.p.slots);
   auto run = [&](auto *t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    if (smem > 32 * 1024)
-      CUDA_TRY(cudaFuncSetAttribute(propose_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    propose_kernel<T><<<(unsigned)a.rows, kThreads, smem, stream>>>(static_cast<const T *>(a.logits), a.vocab, a.topk,
-                                                                    a.order, slots, a.topk_id, a.topk_logp);
+    CUDA_TRY(cudaFuncSetAttribute(propose_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    propose_kernel<T><<<(unsigned)(a.rows * l.p.chunks), kThreads, smem, stream>>>(
+        static_cast<const T *>(a.logits), a.vocab, a.topk, a.order, l.p, reinterpret_cast<SoftSum *>(w + l.part),
+        reinterpret_cast<uint32_t *>(w + l.counts), reinterpret_cast<uint32_t *>(w + l.tickets),
+        reinterpret_cast<Key *>(w + l.kept), a.topk_id, a.topk_logp);
     CUDA_TRY(cudaGetLastError());
   };
   if (a.dtype == FT_DTYPE_F32)

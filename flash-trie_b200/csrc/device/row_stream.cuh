@@ -11,7 +11,10 @@
 namespace ftb {
 
 constexpr float kNegInf = -__builtin_huge_valf();
+// log2(e) as the sum of two floats: one alone is 1.3e-8 off, which would
+// shift every log-sum by that times its mean distance from the maximum.
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2eRest = (float)(1.4426950408889634074 - (double)1.4426950408889634f);
 
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -21,10 +24,10 @@ __device__ __forceinline__ void from_f32(float v, float &o) { o = v; }
 __device__ __forceinline__ void from_f32(float v, __nv_bfloat16 &o) { o = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void from_f32(float v, __half &o) { o = __float2half_rn(v); }
 
-// 2^x; the argument is a difference to a maximum, at most a rounding above 0.
-__device__ __forceinline__ float exp2_fast(float x) {
+// e^d; d is a difference to a maximum, at most a rounding above 0.
+__device__ __forceinline__ float exp_below(float d) {
   float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaf(d, kLog2eRest, d * kLog2e)));
   return y;
 }
 
@@ -83,11 +86,12 @@ struct SoftSum {
 };
 
 __device__ __forceinline__ float exp_from(float x, float m) {
-  return exp2_fast((x - (m == kNegInf ? 0.0f : m)) * kLog2e);
+  return exp_below(x - (m == kNegInf ? 0.0f : m));
 }
 
+// Returns the largest of the values (NaN ones aside).
 template <int N>
-__device__ __forceinline__ void soft_add(SoftSum &s, const float (&v)[N]) {
+__device__ __forceinline__ float soft_add(SoftSum &s, const float (&v)[N]) {
   float top = v[0];
 #pragma unroll
   for (int e = 1; e < N; ++e) top = fmaxf(top, v[e]);
@@ -98,8 +102,9 @@ __device__ __forceinline__ void soft_add(SoftSum &s, const float (&v)[N]) {
   const float base = s.m == kNegInf ? 0.0f : s.m;
   float a = 0.0f;
 #pragma unroll
-  for (int e = 0; e < N; ++e) a += exp2_fast((v[e] - base) * kLog2e);
+  for (int e = 0; e < N; ++e) a += exp_below(v[e] - base);
   s.z += a;
+  return top;
 }
 
 __device__ __forceinline__ SoftSum soft_join(SoftSum a, SoftSum b) {
