@@ -340,10 +340,10 @@ int ft_sequence_grad_device(const ft_sequence_args *args, const float *grad, con
   });
 }
 
-int ft_preference_loss_workspace(const ft_sequence_args *args, uint32_t pairs, uint64_t *bytes) {
+int ft_preference_loss_workspace(const ft_sequence_args *args, uint64_t *bytes) {
   return guarded([&] {
     require_args(args, bytes);
-    *bytes = ftb::preference_workspace(*args, pairs);
+    *bytes = ftb::preference_workspace(*args);
   });
 }
 

@@ -625,7 +625,7 @@ void adapter_logits_device(const ft_adapter_args &a, void *ws, uint64_t ws_bytes
     uint32_t slots = 2;
     while (slots < a.n) slots <<= 1;
     const size_t room = 16ull * slots;
-    if (room > 48 * 1024)
+    if (room > 32 * 1024)
       CUDA_TRY(cudaFuncSetAttribute(order_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)room));
     order_kernel<<<1, 1024, room, stream>>>(a.adapter_ids, a.n, a.num_outpos, a.num_adapters, slots, p.tile_t, o);
     CUDA_TRY(cudaGetLastError());

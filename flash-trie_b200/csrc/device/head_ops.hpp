@@ -20,7 +20,7 @@ void sequence_logp_device(const ft_sequence_args &a, void *ws, uint64_t ws_bytes
 void sequence_grad_device(const ft_sequence_args &a, const float *grad, const float *factor, const float *upstream,
                           void *ws, uint64_t ws_bytes, cudaStream_t stream);
 
-uint64_t preference_workspace(const ft_sequence_args &a, uint32_t pairs);
+uint64_t preference_workspace(const ft_sequence_args &a);
 void preference_loss_device(const ft_sequence_args &a, const ft_preference_args &p, void *ws, uint64_t ws_bytes,
                             cudaStream_t stream);
 

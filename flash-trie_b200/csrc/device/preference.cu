@@ -129,57 +129,72 @@ __device__ double block_sum(double v, double *sm /* [kPairThreads / 32] */) {
   return s;
 }
 
+// Sums of floats that do not depend on the order of the additions: integers in
+// units of a power of two that leaves room for `terms` of them of magnitude
+// below 2^exponent.  For a thousand terms a unit is 2^-51 of that magnitude.
+struct FixedSum {
+  double up, down;
+  __device__ FixedSum(int exponent, uint32_t terms) {
+    const int bits = 62 - (32 - __clz((int)terms)) - exponent;
+    up = scalbn(1.0, bits);
+    down = scalbn(1.0, -bits);
+  }
+  __device__ unsigned long long of(double x) const { return (unsigned long long)__double2ll_rn(x * up); }
+  __device__ double value(unsigned long long s) const { return (double)(long long)s * down; }
+};
+
 // The pairs of one request per CTA: margins, this request's loss and pair
-// count, and each candidate's gradient, summed over the pairs in a fixed
-// order (a warp per candidate, its lanes over the pairs).  The CTA that ends
-// last adds up the requests.
+// count, and each candidate's gradient, added up in shared memory as integers
+// so that it is the same in any order (the weights are below |beta|).  The CTA
+// that ends last adds up the requests.
 __global__ void __launch_bounds__(kPairThreads)
-    pair_kernel(ft_preference_args p, uint32_t n, uint32_t C, const double *logp64, float *coef, double2 *part,
-                uint32_t *ticket) {
+    pair_kernel(ft_preference_args p, uint32_t n, uint32_t C, const double *logp64, double2 *part, uint32_t *ticket) {
+  extern __shared__ unsigned long long acc[];  // [C], then C bits: the candidate is in a pair without a margin
+  uint32_t *broken = reinterpret_cast<uint32_t *>(acc + C);
   __shared__ double sm[kPairThreads / 32];
   __shared__ bool last;
   const uint64_t req = blockIdx.x;
   const double *lp = logp64 + req * C;
   const float *ref = p.ref_logp + req * C;
+  const FixedSum fix(p.beta != 0.0f ? ilogb((double)p.beta) + 1 : 0, 2 * p.pairs);
+  for (uint32_t j = threadIdx.x; j < C; j += kPairThreads) acc[j] = 0;
+  for (uint32_t j = threadIdx.x; j < (C + 31) / 32; j += kPairThreads) broken[j] = 0;
+  __syncthreads();
   double loss = 0.0, count = 0.0;
   for (uint32_t q = threadIdx.x; q < p.pairs; q += kPairThreads) {
     const int32_t c = p.chosen[req * p.pairs + q], r = p.rejected[req * p.pairs + q];
-    float margin = 0.0f, w = 0.0f;
+    float margin = 0.0f;
     if (c >= 0 && r >= 0) {
       count += 1.0;
       if ((uint32_t)c < C && (uint32_t)r < C) {
         const double z = (double)p.beta * ((lp[c] - (double)ref[c]) - (lp[r] - (double)ref[r]));
-        const double e = p.label_smoothing, soft = log1p(exp(-fabs(z)));
+        const double e = p.label_smoothing, t = exp(-fabs(z)), soft = log1p(t);
         const double pos = soft + (z < 0 ? -z : 0.0), neg = soft + (z > 0 ? z : 0.0);
-        const double sig = 1.0 / (1.0 + exp(-z)), gis = 1.0 / (1.0 + exp(z));
+        const double big = 1.0 / (1.0 + t), small = t / (1.0 + t);  // sigmoids of |z| and -|z|
         // A weight of zero takes its side away whatever that side's value.
         loss += (e < 1.0 ? (1.0 - e) * pos : 0.0) + (e > 0.0 ? e * neg : 0.0) + (z != z ? z : 0.0);
         margin = (float)z;
-        w = (float)((double)p.beta * (e * sig - (1.0 - e) * gis));
+        if (z == z) {
+          const double w = (double)p.beta * (e * (z >= 0 ? big : small) - (1.0 - e) * (z >= 0 ? small : big));
+          const unsigned long long u = fix.of(w);
+          atomicAdd(&acc[c], u);
+          atomicAdd(&acc[r], 0ull - u);
+        } else {
+          atomicOr(&broken[(uint32_t)c / 32], 1u << (c % 32));
+          atomicOr(&broken[(uint32_t)r / 32], 1u << (r % 32));
+        }
       } else {
         margin = __int_as_float(0x7FC00000);
         loss += (double)margin;
       }
     }
     p.margin[req * p.pairs + q] = margin;
-    coef[req * p.pairs + q] = w;
   }
   loss = block_sum(loss, sm);
   count = block_sum(count, sm);
-  __syncthreads();  // the block's coef values are visible to all of it
-  const uint32_t lane = threadIdx.x & 31;
-  for (uint32_t j = threadIdx.x >> 5; j < C; j += kPairThreads / 32) {
-    double g = 0.0;
-    for (uint32_t q = lane; q < p.pairs; q += 32) {
-      const int32_t c = p.chosen[req * p.pairs + q], r = p.rejected[req * p.pairs + q];
-      const float w = coef[req * p.pairs + q];
-      if ((uint32_t)c == j) g += w;
-      if ((uint32_t)r == j) g -= w;
-    }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) g += __shfl_xor_sync(~0u, g, d);
-    if (lane == 0) p.grad[req * C + j] = (float)g;
-  }
+  __syncthreads();
+  for (uint32_t j = threadIdx.x; j < C; j += kPairThreads)
+    p.grad[req * C + j] = broken[j / 32] >> (j % 32) & 1 ? __int_as_float(0x7FC00000) : (float)fix.value(acc[j]);
   if (threadIdx.x == 0) {
     part[req] = make_double2(loss, count);
     __threadfence();
@@ -203,75 +218,68 @@ __global__ void __launch_bounds__(kPairThreads)
   }
 }
 
-// One CTA per row: W, and the row's live (token, candidate) pairs sorted, with
-// the summed weight of each distinct token at its first entry.  Adding in the
-// candidates' order keeps the result the same from run to run.
-__global__ void scatter_plan_kernel(const uint32_t *tokens, const int32_t *lengths, const SoftSum *stats, const float *grad,
-                                    const float *factor, const float *upstream, uint32_t vocab, uint32_t L, uint32_t C,
-                                    uint32_t slots, uint32_t *out_tok, float *out_w, uint32_t *out_n, float *out_total) {
-  extern __shared__ unsigned long long key[];
+// One CTA per row: W, and the summed weight of each distinct token of the live
+// candidates.  The tokens meet in a hash table in shared memory (at most half
+// full) whose sums are integers, so that they are the same in any order; the
+// list's order is not, and nothing depends on it.  A weight that is not finite
+// makes W NaN, and with it the row's gradient.
+__global__ void __launch_bounds__(1024)
+    scatter_plan_kernel(const uint32_t *tokens, const int32_t *lengths, const SoftSum *stats, const float *grad,
+                        const float *factor, const float *upstream, uint32_t vocab, uint32_t L, uint32_t C,
+                        uint32_t slots, uint32_t *out_tok, float *out_w, uint32_t *out_n, float *out_total) {
+  extern __shared__ unsigned long long acc[];  // [slots], then u32 [slots] tokens
+  uint32_t *key = reinterpret_cast<uint32_t *>(acc + slots);
   __shared__ double sm[32];
-  __shared__ uint32_t live;
+  __shared__ uint32_t found, largest;
   const uint64_t row = blockIdx.x, req = row / L;
   const uint32_t l = (uint32_t)(row % L);
-  const double scale = (factor ? (double)*factor : 1.0) * (upstream ? (double)*upstream : 1.0);
   const bool dead = stats[row].z == 0.0f;
+  for (uint32_t i = threadIdx.x; i < slots; i += blockDim.x) acc[i] = 0, key[i] = 0xFFFFFFFFu;
+  if (threadIdx.x == 0) found = largest = 0;
+  __syncthreads();
+  auto live = [&](uint32_t j) {
+    const int32_t len = lengths[req * C + j];
+    return !dead && len >= 0 && (uint32_t)len <= L && l < (uint32_t)len;
+  };
   double total = 0.0;
-  if (threadIdx.x == 0) live = 0;
-  __syncthreads();
-  for (uint32_t j = threadIdx.x; j < slots; j += blockDim.x) {
-    unsigned long long k = ~0ull;
-    if (j < C && !dead) {
-      const int32_t len = lengths[req * C + j];
-      if (len >= 0 && (uint32_t)len <= L && l < (uint32_t)len) {
-        const uint32_t t = tokens[(req * C + j) * L + l];
-        total += grad[req * C + j];
-        if (t < vocab) k = ((unsigned long long)t << 32) | j;
-      }
+  uint32_t top = 0;  // of the magnitudes' bits, which compare as the magnitudes do
+  for (uint32_t j = threadIdx.x; j < C; j += blockDim.x)
+    if (live(j)) {
+      const float w = grad[req * C + j];
+      total += w;
+      top = max(top, __float_as_uint(w) & 0x7FFFFFFFu);
     }
-    key[j] = k;
+  top = __reduce_max_sync(~0u, top);
+  if ((threadIdx.x & 31) == 0) atomicMax(&largest, top);
+  total = block_sum(total, sm);  // its barriers make `largest` complete
+  top = largest;
+  const double scale = (factor ? (double)*factor : 1.0) * (upstream ? (double)*upstream : 1.0);
+  if (top >= 0x7F800000u) total = __longlong_as_double(0x7FF8000000000000ll);
+  if (top == 0 || top >= 0x7F800000u) {  // zeros alone, or NaN everywhere
+    if (threadIdx.x == 0) out_n[row] = 0, out_total[row] = (float)(total * scale);
+    return;
   }
-  total = block_sum(total, sm) * scale;
-  for (uint32_t size = 2; size <= slots; size <<= 1)
-    for (uint32_t step = size >> 1; step; step >>= 1) {
-      __syncthreads();
-      for (uint32_t i = threadIdx.x; i < slots / 2; i += blockDim.x) {
-        const uint32_t a = 2 * i - (i & (step - 1)), b = a + step;
-        const bool up = (a & size) == 0;
-        const unsigned long long x = key[a], y = key[b];
-        if ((x > y) == up) key[a] = y, key[b] = x;
+  const FixedSum fix(ilogbf(__uint_as_float(top)) + 1, C);
+  for (uint32_t j = threadIdx.x; j < C; j += blockDim.x)
+    if (live(j)) {
+      const uint32_t t = tokens[(req * C + j) * L + l];
+      if (t >= vocab) continue;
+      uint32_t at = (t * 2654435761u) >> (32 - __popc(slots - 1));
+      for (uint32_t i = 0; i < slots; ++i, at = (at + 1) & (slots - 1)) {
+        const uint32_t was = atomicCAS(&key[at], 0xFFFFFFFFu, t);
+        if (was == 0xFFFFFFFFu || was == t) break;
       }
+      atomicAdd(&acc[at], fix.of(grad[req * C + j]));
     }
   __syncthreads();
-  for (uint32_t i = threadIdx.x; i < C; i += blockDim.x) {
-    const unsigned long long k = key[i];
-    if (k == ~0ull) continue;
-    const uint32_t t = (uint32_t)(k >> 32);
-    if (i + 1 == slots || key[i + 1] == ~0ull) live = i + 1;  // one thread: the last live entry
-    double w = 0.0;
-    if (i == 0 || (uint32_t)(key[i - 1] >> 32) != t)
-      for (uint32_t q = i; q < slots && (uint32_t)(key[q] >> 32) == t && key[q] != ~0ull; ++q)
-        w += grad[req * C + (uint32_t)key[q]];
-    out_tok[row * C + i] = t;
-    out_w[row * C + i] = (float)(w * scale);
-  }
+  for (uint32_t i = threadIdx.x; i < slots; i += blockDim.x)
+    if (key[i] != 0xFFFFFFFFu) {
+      const uint32_t at = atomicAdd(&found, 1u);
+      out_tok[row * C + at] = key[i];
+      out_w[row * C + at] = (float)(fix.value(acc[i]) * scale);
+    }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    out_n[row] = live;
-    out_total[row] = (float)total;
-  }
-}
-
-__device__ uint32_t lower_bound(const uint32_t *a, uint32_t n, uint32_t x) {
-  uint32_t lo = 0;
-  while (n) {
-    const uint32_t h = n / 2;
-    if (a[lo + h] < x)
-      lo += h + 1, n -= h + 1;
-    else
-      n = h;
-  }
-  return lo;
+  if (threadIdx.x == 0) out_n[row] = found, out_total[row] = (float)(total * scale);
 }
 
 __device__ __forceinline__ uint4 pack(const float (&v)[4], const float *) {
@@ -346,11 +354,11 @@ __global__ void __launch_bounds__(kStatThreads)
   const uint32_t *t = tok + row * C;
   const int64_t e0 = max((int64_t)0, out.first(v0)), e1 = min((int64_t)vocab, out.first(v1));
   if (e0 >= e1) return;
-  const uint32_t a = lower_bound(t, n, (uint32_t)e0);
-  for (uint32_t i = a + threadIdx.x; i < n && t[i] < e1; i += kStatThreads) {
-    if (i > 0 && t[i - 1] == t[i]) continue;
-    const float p = zero ? 0.0f : k * exp_below(to_f32(in.row[t[i]]) - base);
-    from_f32(tok_w[row * C + i] + p, g[t[i]]);
+  for (uint32_t i = threadIdx.x; i < n; i += kStatThreads) {
+    const uint32_t at = t[i];
+    if (at < e0 || at >= e1) continue;
+    const float p = zero ? 0.0f : k * exp_below(to_f32(in.row[at]) - base);
+    from_f32(tok_w[row * C + i] + p, g[at]);
   }
 }
 
@@ -405,14 +413,13 @@ uint64_t part_bytes(const ft_sequence_args &a) {
 }
 
 struct PairLayout {
-  uint64_t lp, coef, part, ticket, end;
+  uint64_t lp, part, ticket, end;
 };
 
-PairLayout pair_layout(const ft_sequence_args &a, uint32_t pairs) {
+PairLayout pair_layout(const ft_sequence_args &a) {
   PairLayout l;
   l.lp = part_bytes(a);
-  l.coef = l.lp + align256(8ull * a.n * a.candidates);
-  l.part = l.coef + align256(4ull * a.n * pairs);
+  l.part = l.lp + align256(8ull * a.n * a.candidates);
   l.ticket = l.part + align256(16ull * a.n);
   l.end = l.ticket + 256;
   return l;
@@ -484,11 +491,11 @@ void sequence_grad_device(const ft_sequence_args &a, const float *grad, const fl
   uint32_t *tok = reinterpret_cast<uint32_t *>(w + g.tok), *cnt = reinterpret_cast<uint32_t *>(w + g.n);
   float *tok_w = reinterpret_cast<float *>(w + g.w), *total = reinterpret_cast<float *>(w + g.total);
   const SoftSum *stats = reinterpret_cast<const SoftSum *>(a.stats);
-  uint32_t slots = 2;
-  while (slots < a.candidates) slots <<= 1;
-  const uint32_t threads = std::min<uint32_t>(1024, std::max<uint32_t>(32, slots / 2));
-  const size_t smem = 8ull * slots;
-  if (smem > 48 * 1024)
+  uint32_t slots = 32;
+  while (slots < 2 * a.candidates) slots <<= 1;
+  const uint32_t threads = std::min<uint32_t>(1024, (a.candidates + 31) / 32 * 32);
+  const size_t smem = 12ull * slots;
+  if (smem > 32 * 1024)
     CUDA_TRY(cudaFuncSetAttribute(scatter_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   scatter_plan_kernel<<<(unsigned)p.rows, threads, smem, stream>>>(a.tokens, a.lengths, stats, grad, factor, upstream,
                                                                    a.vocab, a.num_outpos, a.candidates, slots, tok,
@@ -503,9 +510,9 @@ void sequence_grad_device(const ft_sequence_args &a, const float *grad, const fl
   });
 }
 
-uint64_t preference_workspace(const ft_sequence_args &a, uint32_t pairs) {
+uint64_t preference_workspace(const ft_sequence_args &a) {
   check_sequence(a, "preference_loss");
-  return pair_layout(a, pairs).end;
+  return pair_layout(a).end;
 }
 
 void preference_loss_device(const ft_sequence_args &a, const ft_preference_args &p, void *ws, uint64_t ws_bytes,
@@ -513,6 +520,7 @@ void preference_loss_device(const ft_sequence_args &a, const ft_preference_args 
   check_sequence(a, "preference_loss");
   if (!(p.label_smoothing >= 0.0f && p.label_smoothing <= 1.0f))
     throw InvalidArgument("preference_loss: label_smoothing must be in [0, 1]");
+  if (p.pairs >= 1u << 30) throw InvalidArgument("preference_loss: too many pairs per request");
   need_ptr(p.loss, "loss");
   need_ptr(p.factor, "factor");
   if (a.n == 0) {
@@ -528,14 +536,17 @@ void preference_loss_device(const ft_sequence_args &a, const ft_preference_args 
     need_ptr(p.rejected, "rejected");
     need_ptr(p.margin, "margin");
   }
-  const PairLayout l = pair_layout(a, p.pairs);
+  const PairLayout l = pair_layout(a);
   check_room(ws, ws_bytes, l.end, "preference_loss");
   char *w = static_cast<char *>(ws);
   double *lp = reinterpret_cast<double *>(w + l.lp);
   uint32_t *ticket = reinterpret_cast<uint32_t *>(w + l.ticket);
   scores(a, w, lp, ticket, stream);
-  pair_kernel<<<a.n, kPairThreads, 0, stream>>>(p, a.n, a.candidates, lp, reinterpret_cast<float *>(w + l.coef),
-                                                reinterpret_cast<double2 *>(w + l.part), ticket);
+  const size_t smem = 8ull * a.candidates + 4 * ((a.candidates + 31) / 32);
+  if (smem > 32 * 1024)
+    CUDA_TRY(cudaFuncSetAttribute(pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  pair_kernel<<<a.n, kPairThreads, smem, stream>>>(p, a.n, a.candidates, lp, reinterpret_cast<double2 *>(w + l.part),
+                                                   ticket);
   CUDA_TRY(cudaGetLastError());
 }
 

@@ -104,14 +104,14 @@ def _lib():
         lib.ft_trie_device_status.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_uint32)]
         lib.ft_trie_device_status.restype = ctypes.c_int
         lib.ft_last_error.restype = ctypes.c_char_p
-        u64p, vp, u32, u64 = ctypes.POINTER(ctypes.c_uint64), ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint64
+        u64p, vp, u64 = ctypes.POINTER(ctypes.c_uint64), ctypes.c_void_p, ctypes.c_uint64
         for name, args in (("adapter_logits", _AdapterArgs), ("propose", _ProposeArgs),
                            ("sequence_logp", _SequenceArgs)):
             size, call = getattr(lib, "ft_%s_workspace" % name), getattr(lib, "ft_%s_device" % name)
             size.argtypes = [ctypes.POINTER(args), u64p]
             call.argtypes = [ctypes.POINTER(args), vp, u64, vp]
         lib.ft_sequence_grad_device.argtypes = [ctypes.POINTER(_SequenceArgs), vp, vp, vp, vp, u64, vp]
-        lib.ft_preference_loss_workspace.argtypes = [ctypes.POINTER(_SequenceArgs), u32, u64p]
+        lib.ft_preference_loss_workspace.argtypes = [ctypes.POINTER(_SequenceArgs), u64p]
         lib.ft_preference_loss_device.argtypes = [ctypes.POINTER(_SequenceArgs), ctypes.POINTER(_PreferenceArgs), vp,
                                                   u64, vp]
         _LIB = lib
@@ -470,7 +470,7 @@ class _PreferenceLoss(torch.autograd.Function):
         p = _PreferenceArgs(P, int(mean), beta, label_smoothing, ref_logp.data_ptr(), chosen.data_ptr(),
                             rejected.data_ptr(), margin.data_ptr(), loss.data_ptr(), grad.data_ptr(),
                             factor.data_ptr())
-        ws = _workspace(lambda size: _lib().ft_preference_loss_workspace(ctypes.byref(a), P, size), dev)
+        ws = _workspace(lambda size: _lib().ft_preference_loss_workspace(ctypes.byref(a), size), dev)
         _check(_lib().ft_preference_loss_device(ctypes.byref(a), ctypes.byref(p), ctypes.c_void_p(ws.data_ptr()),
                                                 ws.numel(), _raw_stream(dev)))
         ctx.save_for_backward(logits, tokens, lengths, stats, grad, factor)

@@ -348,7 +348,7 @@ typedef struct {
   float *factor;            /* [1]                                */
 } ft_preference_args;
 
-int ft_preference_loss_workspace(const ft_sequence_args *args, uint32_t pairs, uint64_t *bytes);
+int ft_preference_loss_workspace(const ft_sequence_args *args, uint64_t *bytes);
 int ft_preference_loss_device(const ft_sequence_args *args, const ft_preference_args *pref, void *workspace,
                               uint64_t workspace_bytes, void *stream);
 

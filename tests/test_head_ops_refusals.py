@@ -43,9 +43,9 @@ def preference(fd, **kw):
     return fd._PreferenceArgs(**v)
 
 
-def size(fd, name, args, *more):
+def size(fd, name, args):
     out = ctypes.c_uint64(0)
-    rc = getattr(fd._lib(), "ft_%s_workspace" % name)(ctypes.byref(args), *more, ctypes.byref(out))
+    rc = getattr(fd._lib(), "ft_%s_workspace" % name)(ctypes.byref(args), ctypes.byref(out))
     return rc, out.value
 
 
@@ -109,7 +109,7 @@ def test_sequence_shapes_refused(fd, bad):
     a = sequence(fd, **bad)
     lib = fd._lib()
     assert size(fd, "sequence_logp", a)[0] == INVALID
-    assert size(fd, "preference_loss", a, 4)[0] == INVALID
+    assert size(fd, "preference_loss", a)[0] == INVALID
     assert lib.ft_sequence_logp_device(ctypes.byref(a), P, 1 << 60, None) == INVALID
     assert lib.ft_sequence_grad_device(ctypes.byref(a), P, None, None, P, 1 << 60, None) == INVALID
     assert lib.ft_preference_loss_device(ctypes.byref(a), ctypes.byref(preference(fd)), P, 1 << 60, None) == INVALID
@@ -140,6 +140,11 @@ def test_preference_null_refused(fd, bad):
     assert fd._lib().ft_preference_loss_device(ctypes.byref(sequence(fd)), ctypes.byref(p), P, 1 << 40, None) == NULL
 
 
+def test_preference_too_many_pairs_refused(fd):
+    p = preference(fd, pairs=1 << 30)
+    assert fd._lib().ft_preference_loss_device(ctypes.byref(sequence(fd)), ctypes.byref(p), P, 1 << 40, None) == INVALID
+
+
 @pytest.mark.parametrize("eps", [-0.1, 1.5, float("nan")])
 def test_preference_smoothing_refused(fd, eps):
     p = preference(fd, label_smoothing=eps)
@@ -149,11 +154,11 @@ def test_preference_smoothing_refused(fd, eps):
 def test_sequence_workspaces(fd):
     a = sequence(fd)
     lib = fd._lib()
-    for name, more, call in (("sequence_logp", (), lambda ws, have: lib.ft_sequence_logp_device(
+    for name, call in (("sequence_logp", lambda ws, have: lib.ft_sequence_logp_device(
             ctypes.byref(a), ws, have, None)),
-                             ("preference_loss", (4,), lambda ws, have: lib.ft_preference_loss_device(
+                       ("preference_loss", lambda ws, have: lib.ft_preference_loss_device(
                                  ctypes.byref(a), ctypes.byref(preference(fd)), ws, have, None))):
-        rc, need = size(fd, name, a, *more)
+        rc, need = size(fd, name, a)
         assert rc == 0 and need > 0
         assert call(P, 8) == INVALID
         assert call(None, need) == NULL
