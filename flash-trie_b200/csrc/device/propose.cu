@@ -243,15 +243,16 @@ __global__ void __launch_bounds__(kThreads, 2)
   const float bound = sampled ? sample_bound(sh, r, k) : kNegInf;
   __syncthreads();
   SoftSum s = SoftSum::none();
-  auto take = [&](int64_t i, const float (&v)[N]) {
-    if (soft_add(s, v) > bound) {
+  auto keep = [&](int64_t i, const float (&v)[N]) {
 #pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (v[e] > bound) {
-          const uint32_t at = atomicAdd(&sh.count, 1u);
-          if (at < p.cap) list[at] = key_of(v[e], r.first(i) + e);
-        }
-    }
+    for (int e = 0; e < N; ++e)
+      if (v[e] > bound) {
+        const uint32_t at = atomicAdd(&sh.count, 1u);
+        if (at < p.cap) list[at] = key_of(v[e], r.first(i) + e);
+      }
+  };
+  auto take = [&](int64_t i, const float (&v)[N]) {
+    if (soft_add(s, v) > bound) keep(i, v);
   };
   {
     constexpr int U = 4;
@@ -261,11 +262,15 @@ __global__ void __launch_bounds__(kThreads, 2)
         uint4 q[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) q[u] = r.load_whole(i + u * kThreads);
+        float tops[U];
+        if (soft_add<T, U>(s, q, tops) > bound) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          float v[N];
-          unpack(q[u], v, (const T *)nullptr);
-          take(i + u * kThreads, v);
+          for (int u = 0; u < U; ++u)
+            if (tops[u] > bound) {
+              float v[N];
+              unpack(q[u], v, (const T *)nullptr);
+              keep(i + u * kThreads, v);
+            }
         }
       } else {
 #pragma unroll 1
