@@ -48,17 +48,21 @@ struct ProposePlan {
   uint32_t chunks;      // CTAs per row
   uint32_t cap;         // entries that a CTA can keep
   uint32_t emit;        // entries that a CTA hands on
-  uint32_t slots;       // power of two >= k
+  uint32_t slots;       // power of two >= k and 64
   uint64_t vecs_chunk;  // 16-byte vectors per stretch
 };
 
+constexpr uint32_t kFew = 256;  // entries of a bin that are ranked by counting
+
 struct Shared {
   uint32_t hist[kBins];
+  Key few[kFew];
+  Key least;
   uint32_t scan[kThreads / 32];
   Key low[kThreads / 32], high[kThreads / 32];
   SoftSum sums[kThreads / 32];
   SoftSum sum;
-  uint32_t count, bin, above;
+  uint32_t count, bin, above, low32, high32;
   bool last;
 };
 
@@ -135,6 +139,25 @@ __device__ Key keep_largest(Shared &sh, Key *list, uint32_t count, uint32_t k, u
     high = min(high, low + (((Key)1 << shift) - 1));
     need -= above;
     sure += above;
+    if (in_bin <= kFew) {
+      // Each entry of the bin counts those above it: the need-th is the one.
+      if (threadIdx.x == 0) sh.count = 0;
+      __syncthreads();
+      for (uint32_t i = threadIdx.x; i < count; i += kThreads) {
+        const Key x = list[i];
+        if (x >= low && x <= high) sh.few[atomicAdd(&sh.count, 1u)] = x;
+      }
+      __syncthreads();
+      if (threadIdx.x < in_bin) {
+        const Key x = sh.few[threadIdx.x];
+        uint32_t rank = 0;
+        for (uint32_t i = 0; i < in_bin; ++i) rank += sh.few[i] > x;
+        if (rank == need - 1) sh.least = x;
+      }
+      __syncthreads();
+      low = sh.least;
+      break;
+    }
   }
   // In place: a round's entries are read before any is written, and no write
   // goes beyond the entries read so far.
@@ -148,6 +171,51 @@ __device__ Key keep_largest(Shared &sh, Key *list, uint32_t count, uint32_t k, u
   }
   __syncthreads();
   return low;
+}
+
+__device__ __forceinline__ void exchange(Key &x, Key other, bool smaller) {
+  if ((other < x) == smaller) x = other;
+}
+
+// Ascending bitonic sort of list[0, slots), a power of two of at least 64.
+// Steps within 64 entries run in the registers of a warp, two entries a lane.
+__device__ void sort_ascending(Key *list, uint32_t slots) {
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  auto in_warps = [&](uint32_t size, uint32_t last) {  // the steps below 64 of stages size..last
+    for (uint32_t base = warp * 64; base < slots; base += kThreads * 2) {
+      Key x = list[base + lane], y = list[base + lane + 32];
+      for (uint32_t z = size; z <= last; z <<= 1) {
+        if (z >= 64) {
+          const bool up = (base & z) == 0;
+          if ((x > y) == up) {
+            const Key t = x;
+            x = y, y = t;
+          }
+        }
+        for (uint32_t step = min(z, 32u * 2) / 2 == 32 ? 16 : z / 2; step; step >>= 1) {
+          const bool first = (lane & step) == 0;
+          exchange(x, __shfl_xor_sync(~0u, x, step), first == (((base + lane) & z) == 0));
+          exchange(y, __shfl_xor_sync(~0u, y, step), first == (((base + lane + 32) & z) == 0));
+        }
+      }
+      list[base + lane] = x, list[base + lane + 32] = y;
+    }
+    __syncthreads();
+  };
+  __syncthreads();
+  in_warps(2, 64);
+  for (uint32_t size = 128; size <= slots; size <<= 1) {
+    for (uint32_t step = size >> 1; step >= 64; step >>= 1) {
+      for (uint32_t i = threadIdx.x; i < slots / 2; i += kThreads) {
+        const uint32_t a = 2 * i - (i & (step - 1)), b = a + step;
+        const bool up = (a & size) == 0;
+        const Key x = list[a], y = list[b];
+        if ((x > y) == up) list[a] = y, list[b] = x;
+      }
+      __syncthreads();
+    }
+    in_warps(size, size);
+  }
 }
 
 // One stretch with a bound that rises: whenever the next step might not fit,
@@ -188,13 +256,16 @@ __device__ float sample_bound(Shared &sh, const RowVecs<T> &r, uint32_t k) {
   uint32_t key[kLoads][N];
   uint4 q[kLoads];
   int64_t at[kLoads];
+  for (uint32_t b = threadIdx.x; b < kBins; b += kThreads) sh.hist[b] = 0;
+  if (threadIdx.x == 0) sh.low32 = 0xFFFFFFFFu, sh.high32 = 0;
+  __syncthreads();
 #pragma unroll
   for (int u = 0; u < kLoads; ++u) {
     const int64_t seg = u * (kThreads / 32) + (threadIdx.x >> 5);
     at[u] = vecs * seg / kSegments + (threadIdx.x & 31);
     if (r.whole(at[u])) q[u] = r.load_whole(at[u]);
   }
-  Key low = 0xFFFFFFFFu, high = 0;
+  uint32_t low = 0xFFFFFFFFu, high = 0;
 #pragma unroll
   for (int u = 0; u < kLoads; ++u) {
     float v[N];
@@ -205,26 +276,28 @@ __device__ float sample_bound(Shared &sh, const RowVecs<T> &r, uint32_t k) {
 #pragma unroll
     for (int e = 0; e < N; ++e) {
       key[u][e] = v[e] > kNegInf ? ordered(v[e]) : 0;
-      if (key[u][e]) low = min(low, (Key)key[u][e]), high = max(high, (Key)key[u][e]);
+      if (key[u][e]) low = min(low, key[u][e]), high = max(high, key[u][e]);
     }
   }
-  block_range(sh, low, high);
+  low = __reduce_min_sync(~0u, low), high = __reduce_max_sync(~0u, high);
+  if ((threadIdx.x & 31) == 0) atomicMin(&sh.low32, low), atomicMax(&sh.high32, high);
+  __syncthreads();
+  low = sh.low32, high = sh.high32;
   if (high == 0) return kNegInf;
-  const uint32_t span = (uint32_t)(high - low);
+  const uint32_t span = high - low;
   const int bits = 32 - __clz((int)span), shift = bits > 11 ? bits - 11 : 0;
-  clear_bins(sh);
 #pragma unroll
   for (int u = 0; u < kLoads; ++u)
 #pragma unroll
     for (int e = 0; e < N; ++e)
-      if (key[u][e]) atomicAdd(&sh.hist[(key[u][e] - (uint32_t)low) >> shift], 1u);
+      if (key[u][e]) atomicAdd(&sh.hist[(key[u][e] - low) >> shift], 1u);
   // The k-th logit is expected at rank k kSample / V of the sample, give or
   // take its square root; four of them and 8 more are left for safety.
   const float rank = (float)k * kSample / (float)r.len;
   uint32_t bin, above;
   find_bin(sh, (uint32_t)(rank + 4.0f * sqrtf(rank)) + 8, bin, above);
   if (bin == kBins) return kNegInf;
-  return unordered((uint32_t)low + (bin << shift) - 1);  // the bin's least logit still passes
+  return unordered(low + (bin << shift) - 1);  // the bin's least logit still passes
 }
 
 template <typename T>
@@ -314,24 +387,51 @@ __global__ void __launch_bounds__(kThreads, 2)
     __syncthreads();
     if (!sh.last) return;
     __threadfence();
-    if (threadIdx.x == 0) sh.count = 0;
+    // Every thread looks up the same counts (64 at most) and sums.
+    uint32_t total = 0;
     s = SoftSum::none();
-    Key least = 0;
-    for (uint32_t c = 0; c < p.chunks; ++c) {
-      const uint64_t from = row * p.chunks + c;
-      const uint32_t have = __ldcg(&counts[from]);
-      s = soft_join(s, SoftSum{__ldcg(&part[from].m), __ldcg(&part[from].z)});
-      __syncthreads();
-      count = sh.count;
-      if (count + have > p.cap) least = keep_largest(sh, list, count, k, 256);
-      __syncthreads();
-      for (uint32_t i = threadIdx.x; i < have; i += kThreads) {
-        const Key x = __ldcg(&kept[from * p.emit + i]);
-        if (x >= least) list[atomicAdd(&sh.count, 1u)] = x;
+    const uint64_t first = row * p.chunks;
+    if (threadIdx.x < p.chunks) sh.hist[threadIdx.x] = __ldcg(&counts[first + threadIdx.x]);
+    if (threadIdx.x == 0) sh.count = 0;
+    if (threadIdx.x < 32) {
+      for (uint32_t c = threadIdx.x; c < p.chunks; c += 32)
+        s = soft_join(s, SoftSum{__ldcg(&part[first + c].m), __ldcg(&part[first + c].z)});
+#pragma unroll
+      for (int d = 16; d; d >>= 1) {
+        const SoftSum o{__shfl_xor_sync(~0u, s.m, d), __shfl_xor_sync(~0u, s.z, d)};
+        s = soft_join(s, o);
       }
     }
     __syncthreads();
-    count = sh.count;
+    for (uint32_t c = 0; c < p.chunks; ++c) total += sh.hist[c];
+    if (total <= p.cap) {
+      // A warp per stretch, each entry at its place.
+      for (uint32_t c = threadIdx.x >> 5; c < p.chunks; c += kThreads / 32) {
+        uint32_t at = 0;
+        for (uint32_t b = 0; b < c; ++b) at += sh.hist[b];
+        const Key *from = kept + (first + c) * p.emit;
+        const uint32_t have = sh.hist[c];
+#pragma unroll 8
+        for (uint32_t i = threadIdx.x & 31; i < have; i += 32) list[at + i] = __ldcg(&from[i]);
+      }
+      count = total;
+    } else {
+      Key least = 0;
+      for (uint32_t c = 0; c < p.chunks; ++c) {
+        const uint32_t have = __ldcg(&counts[first + c]);
+        __syncthreads();
+        count = sh.count;
+        if (count + have > p.cap) least = keep_largest(sh, list, count, k, 256);
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < have; i += kThreads) {
+          const Key x = __ldcg(&kept[(first + c) * p.emit + i]);
+          if (x >= least) list[atomicAdd(&sh.count, 1u)] = x;
+        }
+      }
+      __syncthreads();
+      count = sh.count;
+    }
+    __syncthreads();
   }
   if (sampled && bound > kNegInf && count < k) {
     careful(sh, list, r, 0, r.count(), k, p.cap);
@@ -354,17 +454,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     list[i] = x;
   }
-  for (uint32_t size = 2; size <= p.slots; size <<= 1)
-    for (uint32_t step = size >> 1; step; step >>= 1) {
-      __syncthreads();
-      for (uint32_t i = threadIdx.x; i < p.slots / 2; i += kThreads) {
-        const uint32_t a = 2 * i - (i & (step - 1)), b = a + step;
-        const bool up = (a & size) == 0;
-        const Key x = list[a], y = list[b];
-        if ((x > y) == up) list[a] = y, list[b] = x;
-      }
-    }
-  __syncthreads();
+  sort_ascending(list, p.slots);
   const float logz = logf(s.z);
   for (uint32_t i = threadIdx.x; i < k; i += kThreads) {
     uint32_t id = 0xFFFFFFFFu;
@@ -400,7 +490,7 @@ struct Layout {
 Layout layout_of(const ft_propose_args &a) {
   Layout l;
   ProposePlan &p = l.p;
-  p.slots = 2;
+  p.slots = 64;
   while (p.slots < a.topk) p.slots <<= 1;
   // Room for what passes the sampled bound: a few thousand entries for small
   // k, about 1.3 k for large (80 KB at k = 1000: two CTAs per SM).

@@ -36,6 +36,7 @@ same stream rules:
     loss, margin = fd.preference_loss(logits, toks, lens, ref, chosen, rejected)  # differentiable
 """
 import ctypes
+import functools
 import math
 import os
 
@@ -283,19 +284,43 @@ def _no_gradient(what, **tensors):
                 raise ValueError("%s has no gradient: detach %s or call it under torch.no_grad()" % (what, name))
 
 
-def _workspace(size_call, device):
-    """The workspace a call asks for, on the current stream."""
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(call, args, *shape):
+    """Bytes that C ABI call `call` asks for at a shape (the leading fields of
+    its argument struct)."""
     need = ctypes.c_uint64(0)
-    _check(size_call(ctypes.byref(need)))
-    return torch.empty(need.value, dtype=torch.uint8, device=device)
+    _check(getattr(_lib(), call)(ctypes.byref(args(*shape)), ctypes.byref(need)))
+    return need.value
+
+
+def _workspace(device, *what):
+    """(tensor, pointer, bytes) of a call's workspace, on the current stream."""
+    need = _workspace_bytes(*what)
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    return ws, ws.data_ptr(), need
 
 
 def _raw_stream(device):
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    return torch.cuda.current_stream(device).cuda_stream
 
 
-def _on(stream, device):
-    return torch.cuda.stream(torch.cuda.current_stream(device) if stream is None else stream)
+class _On:
+    """The call's device and stream made current, where they are not already."""
+
+    def __init__(self, device, stream):
+        self.inner = []
+        if torch.cuda.current_device() != device.index:
+            self.inner.append(torch.cuda.device(device))
+        if stream is not None:
+            self.inner.append(torch.cuda.stream(stream))
+
+    def __enter__(self):
+        for c in self.inner:
+            c.__enter__()
+
+    def __exit__(self, *error):
+        for c in reversed(self.inner):
+            c.__exit__(*error)
 
 
 def adapter_logits(hidden, weight, adapter_ids=None, lora_a=None, lora_b=None, scale=None, out_dtype=None, stream=None):
@@ -343,15 +368,14 @@ def adapter_logits(hidden, weight, adapter_ids=None, lora_a=None, lora_b=None, s
     _no_gradient("adapter_logits", hidden=hidden, weight=weight, lora_a=lora_a, lora_b=lora_b, scale=scale)
     if L == 0 or V == 0 or D == 0:
         raise ValueError("L, V and D must be positive")
-    with torch.cuda.device(dev), _on(stream, dev):
+    shape = (n, L, V, D, r, G, _DTYPE[dt], _DTYPE[out_dtype])
+    with _On(dev, stream):
+        ws, ws_ptr, ws_bytes = _workspace(dev, "ft_adapter_logits_workspace", _AdapterArgs, *shape)
         out = torch.empty((n, L, V), dtype=out_dtype, device=dev)
-        a = _AdapterArgs(n, L, V, D, r, G, _DTYPE[dt], _DTYPE[out_dtype], hidden.data_ptr(), weight.data_ptr(),
-                         adapter_ids.data_ptr() if G else None, lora_a.data_ptr() if G else None,
-                         lora_b.data_ptr() if G else None, scale.data_ptr() if scale is not None else None,
-                         out.data_ptr())
-        ws = _workspace(lambda size: _lib().ft_adapter_logits_workspace(ctypes.byref(a), size), dev)
-        _check(_lib().ft_adapter_logits_device(ctypes.byref(a), ctypes.c_void_p(ws.data_ptr()), ws.numel(),
-                                               _raw_stream(dev)))
+        a = _AdapterArgs(*shape, hidden.data_ptr(), weight.data_ptr(), adapter_ids.data_ptr() if G else None,
+                         lora_a.data_ptr() if G else None, lora_b.data_ptr() if G else None,
+                         scale.data_ptr() if scale is not None else None, out.data_ptr())
+        _check(_lib().ft_adapter_logits_device(ctypes.byref(a), ws_ptr, ws_bytes, _raw_stream(dev)))
     return out
 
 
@@ -379,15 +403,14 @@ def propose(logits, k, order="id", stream=None):
     if V == 0:
         raise ValueError("the vocabulary is empty")
     _no_gradient("propose", logits=logits)
-    with torch.cuda.device(dev), _on(stream, dev):
+    shape = (n * L, V, k, _DTYPE[logits.dtype], int(order == "logp"))
+    with _On(dev, stream):
         ids = torch.empty((n, L, k), dtype=torch.int32, device=dev)
         lps = torch.empty((n, L, k), dtype=torch.float32, device=dev)
         if n * L:
-            a = _ProposeArgs(n * L, V, k, _DTYPE[logits.dtype], int(order == "logp"), logits.data_ptr(),
-                             ids.data_ptr(), lps.data_ptr())
-            ws = _workspace(lambda size: _lib().ft_propose_workspace(ctypes.byref(a), size), dev)
-            _check(_lib().ft_propose_device(ctypes.byref(a), ctypes.c_void_p(ws.data_ptr()), ws.numel(),
-                                            _raw_stream(dev)))
+            ws, ws_ptr, ws_bytes = _workspace(dev, "ft_propose_workspace", _ProposeArgs, *shape)
+            a = _ProposeArgs(*shape, logits.data_ptr(), ids.data_ptr(), lps.data_ptr())
+            _check(_lib().ft_propose_device(ctypes.byref(a), ws_ptr, ws_bytes, _raw_stream(dev)))
     return ids, lps
 
 
@@ -409,79 +432,80 @@ def bs_tbs_hidden(trie, beams, hidden, weight, k, token_logp_threshold, sents_lo
                          early_exit, capacity=capacity, stream=stream, check=check, key_ids=key_ids)
 
 
-def _sequence_args(logits, tokens, lengths, stats, logp=None, grad_logits=None):
+def _sequence_shape(logits, tokens):
     n, L, V = logits.shape
-    return _SequenceArgs(n, L, V, tokens.shape[1], _DTYPE[logits.dtype], 0, logits.data_ptr(), tokens.data_ptr(),
-                         lengths.data_ptr(), stats.data_ptr(), logp.data_ptr() if logp is not None else None,
-                         grad_logits.data_ptr() if grad_logits is not None else None)
+    return n, L, V, tokens.shape[1], _DTYPE[logits.dtype], 0
 
 
 def _sequence_grad(logits, tokens, lengths, stats, grad, factor, upstream):
-    """Gradient of the logits, on the current stream (autograd runs it on the
-    forward call's)."""
+    """Gradient of the logits, on the current stream (autograd makes the
+    forward call's current)."""
     dev = logits.device
-    with torch.cuda.device(dev):
+    with _On(dev, None):
         out = torch.empty_like(logits)
         if logits.numel() == 0 or tokens.shape[1] == 0:
             return out.zero_()
-        a = _sequence_args(logits, tokens, lengths, stats, grad_logits=out)
-        ws = _workspace(lambda size: _lib().ft_sequence_logp_workspace(ctypes.byref(a), size), dev)
-        _check(_lib().ft_sequence_grad_device(
-            ctypes.byref(a), ctypes.c_void_p(grad.data_ptr()),
-            ctypes.c_void_p(factor.data_ptr() if factor is not None else None),
-            ctypes.c_void_p(upstream.data_ptr() if upstream is not None else None), ctypes.c_void_p(ws.data_ptr()),
-            ws.numel(), _raw_stream(dev)))
+        shape = _sequence_shape(logits, tokens)
+        ws, ws_ptr, ws_bytes = _workspace(dev, "ft_sequence_logp_workspace", _SequenceArgs, *shape)
+        a = _SequenceArgs(*shape, logits.data_ptr(), tokens.data_ptr(), lengths.data_ptr(), stats.data_ptr(), None,
+                          out.data_ptr())
+        _check(_lib().ft_sequence_grad_device(ctypes.byref(a), grad.data_ptr(),
+                                              factor.data_ptr() if factor is not None else None,
+                                              upstream.data_ptr() if upstream is not None else None, ws_ptr, ws_bytes,
+                                              _raw_stream(dev)))
     return out
 
 
 class _SequenceLogp(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, lengths):
-        n, L, _ = logits.shape
         dev = logits.device
+        shape = _sequence_shape(logits, tokens)
         logp = torch.empty(lengths.shape, dtype=torch.float32, device=dev)
-        stats = torch.empty((n, L, 2), dtype=torch.float32, device=dev)
+        stats = torch.empty((*shape[:2], 2), dtype=torch.float32, device=dev)
         if logp.numel():
-            a = _sequence_args(logits, tokens, lengths, stats, logp=logp)
-            ws = _workspace(lambda size: _lib().ft_sequence_logp_workspace(ctypes.byref(a), size), dev)
-            _check(_lib().ft_sequence_logp_device(ctypes.byref(a), ctypes.c_void_p(ws.data_ptr()), ws.numel(),
-                                                  _raw_stream(dev)))
+            ws, ws_ptr, ws_bytes = _workspace(dev, "ft_sequence_logp_workspace", _SequenceArgs, *shape)
+            a = _SequenceArgs(*shape, logits.data_ptr(), tokens.data_ptr(), lengths.data_ptr(), stats.data_ptr(),
+                              logp.data_ptr(), None)
+            _check(_lib().ft_sequence_logp_device(ctypes.byref(a), ws_ptr, ws_bytes, _raw_stream(dev)))
         ctx.save_for_backward(logits, tokens, lengths, stats)
         return logp
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        return _sequence_grad(*ctx.saved_tensors, g.to(torch.float32).contiguous(), None, None), None, None
+        return _sequence_grad(*ctx.saved_tensors, g.contiguous(), None, None), None, None
 
 
 class _PreferenceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, lengths, ref_logp, chosen, rejected, beta, label_smoothing, mean):
-        n, L, _ = logits.shape
-        dev, P = logits.device, chosen.shape[1]
-        stats = torch.empty((n, L, 2), dtype=torch.float32, device=dev)
-        margin = torch.empty((n, P), dtype=torch.float32, device=dev)
+        dev = logits.device
+        shape = _sequence_shape(logits, tokens)
+        stats = torch.empty((*shape[:2], 2), dtype=torch.float32, device=dev)
+        margin = torch.empty(chosen.shape, dtype=torch.float32, device=dev)
         # Two tensors: a caller may change the loss in place before the backward pass.
         loss = torch.empty((), dtype=torch.float32, device=dev)
         factor = torch.empty((), dtype=torch.float32, device=dev)
         grad = torch.empty(ref_logp.shape, dtype=torch.float32, device=dev)
-        a = _sequence_args(logits, tokens, lengths, stats)
-        p = _PreferenceArgs(P, int(mean), beta, label_smoothing, ref_logp.data_ptr(), chosen.data_ptr(),
+        ws, ws_ptr, ws_bytes = _workspace(dev, "ft_preference_loss_workspace", _SequenceArgs, *shape)
+        a = _SequenceArgs(*shape, logits.data_ptr(), tokens.data_ptr(), lengths.data_ptr(), stats.data_ptr(), None, None)
+        p = _PreferenceArgs(chosen.shape[1], int(mean), beta, label_smoothing, ref_logp.data_ptr(), chosen.data_ptr(),
                             rejected.data_ptr(), margin.data_ptr(), loss.data_ptr(), grad.data_ptr(),
                             factor.data_ptr())
-        ws = _workspace(lambda size: _lib().ft_preference_loss_workspace(ctypes.byref(a), size), dev)
-        _check(_lib().ft_preference_loss_device(ctypes.byref(a), ctypes.byref(p), ctypes.c_void_p(ws.data_ptr()),
-                                                ws.numel(), _raw_stream(dev)))
+        _check(_lib().ft_preference_loss_device(ctypes.byref(a), ctypes.byref(p), ws_ptr, ws_bytes, _raw_stream(dev)))
         ctx.save_for_backward(logits, tokens, lengths, stats, grad, factor)
         ctx.mark_non_differentiable(margin)
+        ctx.set_materialize_grads(False)  # the margin's is not looked at
         return loss, margin
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g, _):
+        if g is None:
+            return (None,) * 9
         *saved, grad, factor = ctx.saved_tensors
-        return (_sequence_grad(*saved, grad, factor, g.to(torch.float32).contiguous()),) + (None,) * 8
+        return (_sequence_grad(*saved, grad, factor, g),) + (None,) * 8
 
 
 def _want_candidates(logits, tokens, lengths):
@@ -513,7 +537,7 @@ def sequence_logp(logits, tokens, lengths, stream=None):
     all -inf, has log-probability -inf.  The gradient is deterministic; the
     backward pass runs on the forward call's stream."""
     dev = _want_candidates(logits, tokens, lengths)
-    with torch.cuda.device(dev), _on(stream, dev):
+    with _On(dev, stream):
         return _SequenceLogp.apply(logits, tokens, lengths)
 
 
@@ -552,6 +576,6 @@ def preference_loss(logits, tokens, lengths, ref_logp, chosen, rejected, beta=0.
         raise ValueError("label_smoothing must be in [0, 1]")
     if reduction not in ("mean", "sum"):
         raise ValueError("reduction must be 'mean' or 'sum'")
-    with torch.cuda.device(dev), _on(stream, dev):
+    with _On(dev, stream):
         return _PreferenceLoss.apply(logits, tokens, lengths, ref_logp, chosen, rejected, beta, label_smoothing,
                                      reduction == "mean")
