@@ -9,9 +9,11 @@
 // the proposals from the rest.
 //
 // The logits are read once.  A row is cut into stretches, a CTA each.  A
-// sample spread over the row gives a bound that about 8 + k + 4 sqrt entries
-// in the sample's measure pass; the CTA streams its stretch, adds to the
-// softmax sum and keeps what passes the bound in shared memory.  The CTA that
+// sample spread over the row gives a bound that a little more than k entries
+// should pass; the CTA streams its stretch, adds to the
+// softmax sum and notes the vectors in which something passes the bound (noting
+// takes a few instructions, taking the entries out at once a fifth of the
+// stream's time); then it fetches those again and keeps what passes.  The CTA that
 // ends last in its row joins the sums, selects the k largest of what all have
 // kept, and sorts them.  The bound is a guess only: a stretch that keeps more
 // than fits is read again with a bound that rises (`careful`), and a row that
@@ -29,7 +31,6 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr uint32_t kBins = 2048;
-constexpr uint32_t kSample = 8192;  // sampled entries of a row
 constexpr float kFltMax = 3.402823466e+38f;
 
 typedef unsigned long long Key;
@@ -47,6 +48,7 @@ __device__ __forceinline__ Key key_of(float x, int64_t id) { return (Key)ordered
 struct ProposePlan {
   uint32_t chunks;      // CTAs per row
   uint32_t cap;         // entries that a CTA can keep
+  uint32_t hits;        // vectors that it can note
   uint32_t emit;        // entries that a CTA hands on
   uint32_t slots;       // power of two >= k and 64
   uint64_t vecs_chunk;  // 16-byte vectors per stretch
@@ -62,7 +64,7 @@ struct Shared {
   Key low[kThreads / 32], high[kThreads / 32];
   SoftSum sums[kThreads / 32];
   SoftSum sum;
-  uint32_t count, bin, above, low32, high32;
+  uint32_t count, hits, bin, above, low32, high32;
   bool last;
 };
 
@@ -247,12 +249,16 @@ __device__ void careful(Shared &sh, Key *list, const RowVecs<T> &r, int64_t v0, 
   __syncthreads();
 }
 
-// A bound below the row's k-th largest logit, from a sample of it (warps read
-// stretches of 32 vectors spread evenly over the row).
+// A bound below the row's k-th largest logit, from a sample of it: groups of
+// eight vectors in the middle of equal parts of the row. Small parts matter: a
+// vocabulary in order of frequency has its best logits at one end, and with
+// long stretches the sample would see too many of them or none; single vectors
+// cost three times as much to fetch.
 template <typename T>
 __device__ float sample_bound(Shared &sh, const RowVecs<T> &r, uint32_t k) {
-  constexpr int N = RowVecs<T>::N, kLoads = kSample / N / kThreads, kSegments = kLoads * kThreads / 32;
+  constexpr int N = RowVecs<T>::N, kLoads = 4;
   const int64_t vecs = r.count();
+  const int loads = (int)max((int64_t)1, min((int64_t)kLoads, vecs / (2 * kThreads))), parts = loads * kThreads / 8;
   uint32_t key[kLoads][N];
   uint4 q[kLoads];
   int64_t at[kLoads];
@@ -261,8 +267,8 @@ __device__ float sample_bound(Shared &sh, const RowVecs<T> &r, uint32_t k) {
   __syncthreads();
 #pragma unroll
   for (int u = 0; u < kLoads; ++u) {
-    const int64_t seg = u * (kThreads / 32) + (threadIdx.x >> 5);
-    at[u] = vecs * seg / kSegments + (threadIdx.x & 31);
+    const int64_t part = (u * kThreads + (int)threadIdx.x) / 8;
+    at[u] = u < loads ? vecs * (2 * part + 1) / (2 * parts) + threadIdx.x % 8 : vecs;  // vecs: nothing
     if (r.whole(at[u])) q[u] = r.load_whole(at[u]);
   }
   uint32_t low = 0xFFFFFFFFu, high = 0;
@@ -291,11 +297,12 @@ __device__ float sample_bound(Shared &sh, const RowVecs<T> &r, uint32_t k) {
 #pragma unroll
     for (int e = 0; e < N; ++e)
       if (key[u][e]) atomicAdd(&sh.hist[(key[u][e] - low) >> shift], 1u);
-  // The k-th logit is expected at rank k kSample / V of the sample, give or
-  // take its square root; four of them and 8 more are left for safety.
-  const float rank = (float)k * kSample / (float)r.len;
+  // The k-th logit is expected at rank k (sample size) / V of the sample, give or
+  // take its square root; four of them and 4 more are left for safety (a row
+  // for which that is too few is read again).
+  const float rank = (float)k * (float)(loads * kThreads * N) / (float)r.len;
   uint32_t bin, above;
-  find_bin(sh, (uint32_t)(rank + 4.0f * sqrtf(rank)) + 8, bin, above);
+  find_bin(sh, (uint32_t)(rank + 4.0f * sqrtf(rank)) + 4, bin, above);
   if (bin == kBins) return kNegInf;
   return unordered(low + (bin << shift) - 1);  // the bin's least logit still passes
 }
@@ -304,31 +311,27 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads, 2)
     propose_kernel(const T *logits, uint32_t vocab, uint32_t k, int order, ProposePlan p, SoftSum *part, uint32_t *counts,
                    uint32_t *tickets, Key *kept, uint32_t *out_id, float *out_lp) {
-  extern __shared__ Key list[];  // [max(cap, slots)]
+  extern __shared__ Key list[];  // [cap], then u32 [hits]
+  uint32_t *hit = reinterpret_cast<uint32_t *>(list + p.cap);
   __shared__ Shared sh;
   constexpr int N = RowVecs<T>::N;
   const uint64_t row = blockIdx.x / p.chunks;
   const uint32_t chunk = blockIdx.x % p.chunks;
   const RowVecs<T> r(logits + row * vocab, vocab);
   const int64_t v0 = (int64_t)(chunk * p.vecs_chunk), v1 = min(v0 + (int64_t)p.vecs_chunk, r.count());
-  if (threadIdx.x == 0) sh.count = 0;
+  if (threadIdx.x == 0) sh.count = sh.hits = 0;
   const bool sampled = vocab > p.cap;
   const float bound = sampled ? sample_bound(sh, r, k) : kNegInf;
   __syncthreads();
   SoftSum s = SoftSum::none();
-  auto keep = [&](int64_t i, const float (&v)[N]) {
-#pragma unroll
-    for (int e = 0; e < N; ++e)
-      if (v[e] > bound) {
-        const uint32_t at = atomicAdd(&sh.count, 1u);
-        if (at < p.cap) list[at] = key_of(v[e], r.first(i) + e);
-      }
-  };
-  auto take = [&](int64_t i, const float (&v)[N]) {
-    if (soft_add(s, v) > bound) keep(i, v);
+  auto note = [&](int64_t i, float top) {
+    if (top > bound) {
+      const uint32_t at = atomicAdd(&sh.hits, 1u);
+      if (at < p.hits) hit[at] = (uint32_t)(i - v0);
+    }
   };
   {
-    constexpr int U = 4;
+    constexpr int U = 8;  // 128 KB on their way per SM; 4 is 6% slower on f32, a third CTA per SM (spills) 30%
     int64_t i = v0 + threadIdx.x;
     for (; i + (U - 1) * kThreads < v1; i += U * kThreads) {
       if (r.whole(i) && r.whole(i + (U - 1) * kThreads)) {
@@ -338,19 +341,14 @@ __global__ void __launch_bounds__(kThreads, 2)
         float tops[U];
         if (soft_add<T, U>(s, q, tops) > bound) {
 #pragma unroll
-          for (int u = 0; u < U; ++u)
-            if (tops[u] > bound) {
-              float v[N];
-              unpack(q[u], v, (const T *)nullptr);
-              keep(i + u * kThreads, v);
-            }
+          for (int u = 0; u < U; ++u) note(i + u * kThreads, tops[u]);
         }
       } else {
 #pragma unroll 1
         for (int u = 0; u < U; ++u) {
           float v[N];
           r.load_edge(i + u * kThreads, v);
-          take(i + u * kThreads, v);
+          note(i + u * kThreads, soft_add(s, v));
         }
       }
     }
@@ -360,12 +358,29 @@ __global__ void __launch_bounds__(kThreads, 2)
         unpack(r.load_whole(i), v, (const T *)nullptr);
       else
         r.load_edge(i, v);
-      take(i, v);
+      note(i, soft_add(s, v));
     }
   }
-  s = soft_join_block<kThreads>(s, sh.sums);  // a barrier: the list is complete
+  s = soft_join_block<kThreads>(s, sh.sums);  // a barrier: all hits are noted
+  const uint32_t hits = sh.hits;
+  if (hits <= p.hits)
+    for (uint32_t h = threadIdx.x; h < hits; h += kThreads) {
+      const int64_t i = v0 + hit[h];
+      float v[N];
+      if (r.whole(i))
+        unpack(r.load_whole(i), v, (const T *)nullptr);
+      else
+        r.load_edge(i, v);
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (v[e] > bound) {
+          const uint32_t at = atomicAdd(&sh.count, 1u);
+          if (at < p.cap) list[at] = key_of(v[e], r.first(i) + e);
+        }
+    }
+  __syncthreads();
   uint32_t count = sh.count;
-  if (count > p.cap) {
+  if (hits > p.hits || count > p.cap) {
     careful(sh, list, r, v0, v1, k, p.cap);
     count = sh.count;
   }
@@ -493,8 +508,10 @@ Layout layout_of(const ft_propose_args &a) {
   p.slots = 64;
   while (p.slots < a.topk) p.slots <<= 1;
   // Room for what passes the sampled bound: a few thousand entries for small
-  // k, about 1.3 k for large (80 KB at k = 1000: two CTAs per SM).
-  p.cap = 8192 + 2 * a.topk;
+  // k, up to 1.9 k for large; 96 KB at k = 1000, so that two CTAs fit on an SM.
+  // `careful` needs room for topk + 256 and a step of all threads.
+  p.cap = std::max(a.topk + 512 + kThreads * 8, 2 * a.topk + 4096);
+  p.hits = std::min(4096 + a.topk / 2 * 3, (uint32_t)(225 * 1024 - sizeof(Shared) - 8 * p.cap) / 4);
   p.emit = a.topk + 4096;  // cap - emit >= topk: a list that lacks room for another has topk entries
   const uint64_t vecs = ((uint64_t)a.vocab * (a.dtype == FT_DTYPE_F32 ? 4 : 2) + 15) / 16 + 1;
   const uint64_t slots = 148 * 2;
@@ -530,7 +547,7 @@ void propose_device(const ft_propose_args &a, void *ws, uint64_t ws_bytes, cudaS
     throw InvalidArgument("propose: needs a 256-byte aligned workspace of " + std::to_string(l.end) + " bytes");
   uint8_t *w = static_cast<uint8_t *>(ws);
   if (l.p.chunks > 1) CUDA_TRY(cudaMemsetAsync(w + l.tickets, 0, 4 * a.rows, stream));
-  const size_t smem = 8ull * std::max(l.p.cap, l.p.slots);
+  const size_t smem = 8ull * l.p.cap + 4ull * l.p.hits;
   auto run = [&](auto *t) {
     using T = std::remove_pointer_t<decltype(t)>;
     CUDA_TRY(cudaFuncSetAttribute(propose_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
