@@ -15,9 +15,9 @@
 // adds its u B^T to its own columns with further tensor products; u goes in as
 // two or three 16-bit parts, so that no more than 2^-18 of it is lost (2^-27
 // for f32 logits).  No column is shared, so an adapter with infinities reaches
-// no other one's requests.  "Direct": the tokens stay as they are and the
-// epilogue adds the products in 32 bits, for batches whose groups are so small
-// that padding them would cost more.
+// no other one's requests.  "Direct": the tokens stay as they are, a kernel of
+// its own makes the low-rank part in 32 bits and the epilogue adds it, for
+// batches whose groups are so small that padding them would cost more.
 #include <algorithm>
 #include <string>
 
@@ -46,6 +46,9 @@ __device__ __forceinline__ void unpack8(uint4 q, float (&v)[8]) {
   unpack(q, v, (const T *)nullptr);
 }
 
+// A group has at least 16 columns, so that a tile has 16 groups at most.
+constexpr uint32_t kTileGroups = kMaxTileT / 16 + 1;
+
 struct Group {
   int32_t adapter;  // -1: none
   uint32_t col0, col1, pad;
@@ -56,12 +59,14 @@ struct Sorted {
   uint32_t *head;        // [0] groups, [1] columns
   Group *groups;
   uint32_t *tile_first;  // first group of each tile of tokens
+  Group *tile_groups;    // [tiles][kTileGroups]: the groups with columns in a tile, then one that begins nowhere
   uint32_t *req_col;     // first column of each request
   int32_t *col_token;    // token of a column; -1 padding; -2 - token: of a request whose adapter does not exist
   void *hidden;          // [columns][dim]
-  void *u;               // [parts][columns][rank]
+  uint8_t *u;            // [rank / width][columns / 8][parts][8 columns][width], swizzled as in shared memory
   uint32_t columns;      // upper bound, a multiple of 16
   uint32_t parts;
+  uint32_t width;        // low-rank rows that a product's operands hold side by side: 16, 32 or 64
 };
 
 // Sum over the items of the threads before this one, and over all.
@@ -140,6 +145,14 @@ __global__ void __launch_bounds__(1024) order_kernel(const int32_t *ids, uint32_
   }
   if (threadIdx.x == 0) o.head[0] = groups, o.head[1] = columns;
   __syncthreads();
+  for (uint32_t q = p0; q < p0 + per && q < groups; ++q) {
+    const Group mine = o.groups[q];
+    for (uint32_t t = mine.col0 / tile_t; t * tile_t < mine.col1; ++t) {
+      const uint32_t at = t * kTileGroups + q - o.tile_first[t];
+      o.tile_groups[at] = mine;
+      if (mine.col1 >= (t + 1) * tile_t || q + 1 == groups) o.tile_groups[at + 1] = Group{-1, ~0u, ~0u, 0};
+    }
+  }
   g = g_before;  // groups that begin before this thread's positions
   for (uint32_t i = p0; i < p0 + per && i < n; ++i) {
     if (head(i)) ++g;
@@ -147,11 +160,12 @@ __global__ void __launch_bounds__(1024) order_kernel(const int32_t *ids, uint32_
   }
 }
 
-constexpr int kShrinkTokens = 4;
+constexpr int kShrinkTokens = 4, kShrinkRows = 4;
 
-// u of up to four tokens of a request: a warp per low-rank row, its lanes over
-// the inner dimension.  The sorted form also moves the tokens to their columns
-// and splits u into 16-bit parts.
+// u of up to four tokens of a request: a warp takes four low-rank rows, its
+// lanes the inner dimension. The sorted form also moves the tokens to their
+// columns and splits u into 16-bit parts, laid out as the products read them,
+// the parts of eight columns next to one another.
 template <typename T, bool kSorted>
 __global__ void __launch_bounds__(256) shrink_kernel(ft_adapter_args a, float *u, Sorted o) {
   const uint32_t per = (a.num_outpos + kShrinkTokens - 1) / kShrinkTokens;
@@ -174,40 +188,60 @@ __global__ void __launch_bounds__(256) shrink_kernel(ft_adapter_args a, float *u
     }
     if (!has) return;  // its columns take no part in any group's products
   }
-  for (uint32_t r = threadIdx.x >> 5; r < a.rank; r += 8) {
-    float s[kShrinkTokens] = {};
-    if (has) {
+  const float scale = has && a.scale ? a.scale[id] : 1.0f;
+  // Rows up to the next multiple of 16 exist as zeros in the sorted form.
+  const uint32_t rows = kSorted ? (a.rank + 15) / 16 * 16 : a.rank;
+  for (uint32_t r = (threadIdx.x >> 5) * kShrinkRows; r < rows; r += 8 * kShrinkRows) {
+    float s[kShrinkRows][kShrinkTokens] = {};
+    if (has && r < a.rank) {
       const T *w = static_cast<const T *>(a.lora_a) + ((uint64_t)id * a.rank + r) * a.dim;
       for (uint32_t d = lane * 8; d < a.dim; d += 256) {
-        float y[8];
-        unpack8<T>(__ldg(reinterpret_cast<const uint4 *>(w + d)), y);
+        uint4 wq[kShrinkRows], xq[kShrinkTokens];
+#pragma unroll
+        for (int i = 0; i < kShrinkRows; ++i) wq[i] = __ldg(reinterpret_cast<const uint4 *>(w + (uint64_t)i * a.dim + d));
+#pragma unroll
+        for (int q = 0; q < kShrinkTokens; ++q)
+          xq[q] = __ldg(reinterpret_cast<const uint4 *>(h + (uint64_t)min(q, (int)count - 1) * a.dim + d));
 #pragma unroll
         for (int q = 0; q < kShrinkTokens; ++q) {
-          if (q >= (int)count) break;
           float x[8];
-          unpack8<T>(__ldg(reinterpret_cast<const uint4 *>(h + (uint64_t)q * a.dim + d)), x);
+          unpack8<T>(xq[q], x);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) s[q] = fmaf(x[e], y[e], s[q]);
+          for (int i = 0; i < kShrinkRows; ++i) {
+            float y[8];
+            unpack8<T>(wq[i], y);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[i][q] = fmaf(x[e], y[e], s[i][q]);
+          }
         }
       }
 #pragma unroll
-      for (int q = 0; q < kShrinkTokens; ++q) {
+      for (int i = 0; i < kShrinkRows; ++i)
 #pragma unroll
-        for (int d = 16; d; d >>= 1) s[q] += __shfl_xor_sync(~0u, s[q], d);
-        s[q] *= a.scale ? a.scale[id] : 1.0f;
-      }
+        for (int q = 0; q < kShrinkTokens; ++q) {
+#pragma unroll
+          for (int d = 16; d; d >>= 1) s[i][q] += __shfl_xor_sync(~0u, s[i][q], d);
+          s[i][q] *= scale;
+        }
     }
-    if (lane < count) {
-      float v = s[0];
+    if (lane < count * kShrinkRows) {  // lane: token lane / 4, row r + lane % 4
+      const uint32_t q = lane / kShrinkRows, i = lane % kShrinkRows;
+      float v = 0.0f;
 #pragma unroll
-      for (int q = 1; q < kShrinkTokens; ++q) v = lane == q ? s[q] : v;
+      for (int x = 0; x < kShrinkRows; ++x)
+#pragma unroll
+        for (int y = 0; y < kShrinkTokens; ++y)
+          if (i == x && q == y) v = s[x][y];
       if (!kSorted) {
-        u[(tok + lane) * a.rank + r] = v;
+        u[(tok + q) * a.rank + r + i] = v;
       } else {
+        const uint32_t c = col + q, row = o.width * 2;
+        uint8_t *at = o.u + ((uint64_t)((r + i) / o.width) * (o.columns / 8) + c / 8) * o.parts * 8 * row +
+                      sm100::swizzled(c % 8 * row + (r + i) % o.width * 2, row);
         for (uint32_t part = 0; part < o.parts; ++part) {
           T x;
           from_f32(v, x);
-          static_cast<T *>(o.u)[((uint64_t)part * o.columns + col + lane) * a.rank + r] = x;
+          *reinterpret_cast<T *>(at + part * 8 * row) = x;
           // What is left for the next part; nothing behind an infinity.
           const float back = to_f32(x);
           v = fabsf(back) < -kNegInf ? v - back : 0.0f;
@@ -217,55 +251,107 @@ __global__ void __launch_bounds__(256) shrink_kernel(ft_adapter_args a, float *u
   }
 }
 
+constexpr int kExpandThreads = 256, kExpandTokens = 8;
+
+// The direct form's low-rank part: one vocabulary entry per thread for the
+// tokens of one request, so that an adapter's rows are read once a request.
+template <typename T>
+__global__ void __launch_bounds__(kExpandThreads) expand_kernel(ft_adapter_args a, const float *u, float *delta) {
+  const uint32_t blocks = (a.vocab + kExpandThreads - 1) / kExpandThreads;
+  const uint32_t req = blockIdx.x / blocks, v = blockIdx.x % blocks * kExpandThreads + threadIdx.x;
+  const int32_t id = a.adapter_ids[req];
+  if ((uint32_t)id >= a.num_adapters || v >= a.vocab) return;
+  const T *b = static_cast<const T *>(a.lora_b) + ((uint64_t)id * a.vocab + v) * a.rank;
+  for (uint32_t l0 = 0; l0 < a.num_outpos; l0 += kExpandTokens) {
+    const uint64_t t0 = (uint64_t)req * a.num_outpos + l0;
+    const uint32_t count = min((uint32_t)kExpandTokens, a.num_outpos - l0);
+    float acc[kExpandTokens] = {};
+#pragma unroll 2
+    for (uint32_t r = 0; r < a.rank; r += 8) {
+      float w[8];
+      unpack8<T>(__ldg(reinterpret_cast<const uint4 *>(b + r)), w);
+#pragma unroll
+      for (int q = 0; q < kExpandTokens; ++q) {
+        if (q >= (int)count) break;
+        const float4 *x = reinterpret_cast<const float4 *>(u + (t0 + q) * a.rank + r);
+        const float4 x0 = __ldg(x), x1 = __ldg(x + 1);
+        float s = acc[q];
+        s = fmaf(x0.x, w[0], s), s = fmaf(x0.y, w[1], s), s = fmaf(x0.z, w[2], s), s = fmaf(x0.w, w[3], s);
+        s = fmaf(x1.x, w[4], s), s = fmaf(x1.y, w[5], s), s = fmaf(x1.z, w[6], s), s = fmaf(x1.w, w[7], s);
+        acc[q] = s;
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < kExpandTokens; ++q)
+      if (q < (int)count) delta[(t0 + q) * a.vocab + v] = acc[q];
+  }
+}
+
 struct LogitsPlan {
   uint32_t columns;    // tokens, or the sorted form's upper bound
   uint32_t tile_t;     // columns of a tile, a multiple of 16
   uint32_t tiles_t;
   uint32_t tiles_v;
+  uint32_t slot_t;     // rows that a stage has for them
   uint32_t stages;
   uint32_t tmem_half;  // columns of one of the two accumulators
 };
 
 struct alignas(8) LogitsShared {
   uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
+  Group list[2][kTileGroups];  // of the tile that loads and products are at
   uint32_t tmem, gave_up;
 };
 
-LogitsPlan plan_logits(const ft_adapter_args &a, uint32_t columns) {
+LogitsPlan plan_logits(const ft_adapter_args &a, uint32_t columns, uint32_t parts) {
   LogitsPlan p;
   p.columns = columns;
   p.tiles_t = (columns + kMaxTileT - 1) / kMaxTileT;
   p.tile_t = ((columns + p.tiles_t - 1) / p.tiles_t + 15) / 16 * 16;
   p.tiles_v = (a.vocab + kTileV - 1) / kTileV;
-  const uint32_t stage = (kTileV + p.tile_t) * kTileD * 2;
+  p.slot_t = std::max(p.tile_t, 16 * parts);
+  const uint32_t stage = (kTileV + p.slot_t) * kTileD * 2;
   p.stages = std::min<uint32_t>(kMaxStages, (225 * 1024) / stage);
   p.tmem_half = 32;
   while (p.tmem_half < p.tile_t) p.tmem_half *= 2;
   return p;
 }
-size_t logits_smem(const LogitsPlan &p) { return 1024 + (size_t)p.stages * (kTileV + p.tile_t) * kTileD * 2; }
+size_t logits_smem(const LogitsPlan &p) { return 1024 + (size_t)p.stages * (kTileV + p.slot_t) * kTileD * 2; }
 
 // The stages of a tile in the order that loads and products both take them:
 // the shared projection's, then those of each group that has columns in it.
-// f(chunk) for the first; g(group, first column, width, rank offset, first
-// part, parts) for the others.  A callback that returns false ends the walk.
-template <typename F, typename G>
-__device__ __forceinline__ bool walk_tile(const ft_adapter_args &a, const Sorted &o, bool sorted, uint32_t tile_t,
-                                          uint32_t groups, uint32_t tt, uint32_t chunks, F &&f, G &&g) {
+// f(chunk) for the first, a stage each. The others share stages as far as they
+// fit: g(adapter, first column, width, low-rank slice, offset in the stage),
+// with open() before the first of a stage and close() after the last. A
+// callback that returns false ends the walk.
+template <typename F, typename Open, typename G, typename Close>
+__device__ __forceinline__ bool walk_tile(const ft_adapter_args &a, const LogitsPlan &p, const Sorted &o, bool sorted,
+                                          const Group *list, uint32_t tt, uint32_t chunks, F &&f, Open &&open, G &&g,
+                                          Close &&close) {
   for (uint32_t c = 0; c < chunks; ++c)
     if (!f(c)) return false;
   if (!sorted) return true;
-  const uint32_t c0 = tt * tile_t, c1 = c0 + tile_t;
-  for (uint32_t i = o.tile_first[tt]; i < groups; ++i) {
-    const Group q = o.groups[i];
-    if (q.col0 >= c1) break;
+  const uint32_t c0 = tt * p.tile_t, c1 = c0 + p.tile_t, room = (kTileV + p.slot_t) * kTileD * 2;
+  const uint32_t fixed = kTileV * o.width * 2, each = o.parts * o.width * 2;  // bytes of B, and of u per column
+  const uint32_t most = (room - fixed) / each / 16 * 16;
+  uint32_t used = 0;
+  for (uint32_t i = 0; list[i].col0 < c1; ++i) {
+    const Group q = list[i];
     if (q.adapter < 0) continue;
-    const uint32_t w0 = max(q.col0, c0), w = min(q.col1, c1) - w0;
-    const uint32_t at_once = min(o.parts, tile_t / w);
-    for (uint32_t r = 0; r < a.rank; r += kTileD)
-      for (uint32_t part = 0; part < o.parts; part += at_once)
-        if (!g(q.adapter, w0, w, r, part, min(at_once, o.parts - part))) return false;
+    const uint32_t end = min(q.col1, c1);
+    for (uint32_t w0 = max(q.col0, c0); w0 < end; w0 += most)
+      for (uint32_t j = 0; j * o.width < a.rank; ++j) {
+        const uint32_t w = min(most, end - w0), need = fixed + w * each;
+        if (used && used + need > room) {
+          close();
+          used = 0;
+        }
+        if (!used && !open()) return false;
+        g(q.adapter, w0, w, j, used);
+        used += need;
+      }
   }
+  if (used) close();
   return true;
 }
 
@@ -274,15 +360,14 @@ __device__ __forceinline__ bool walk_tile(const ft_adapter_args &a, const Sorted
 template <typename T, typename O, bool kSorted>
 __global__ void __launch_bounds__(kThreads, 1)
     logits_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_h,
-                  const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_u,
-                  ft_adapter_args a, LogitsPlan p, const float *u, Sorted o) {
+                  const __grid_constant__ CUtensorMap map_b, ft_adapter_args a, LogitsPlan p, const float *delta, Sorted o) {
   using namespace sm100;
   extern __shared__ uint8_t raw[];
   uint8_t *buf = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   __shared__ LogitsShared sh;
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t bytes_w = kTileV * kTileD * 2, bytes = bytes_w + p.tile_t * kTileD * 2;
-  const uint32_t groups = kSorted ? o.head[0] : 0, columns = kSorted ? o.head[1] : p.columns;
+  const uint32_t warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const uint32_t bytes_w = kTileV * kTileD * 2, bytes = bytes_w + p.slot_t * kTileD * 2;
+  const uint32_t columns = kSorted ? o.head[1] : p.columns;
   const uint32_t tiles_t = (columns + p.tile_t - 1) / p.tile_t;
   const uint32_t tiles = tiles_t * p.tiles_v, chunks = (a.dim + kTileD - 1) / kTileD;
   volatile uint32_t *gave_up = &sh.gave_up;
@@ -300,95 +385,133 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_after();
   const uint32_t tmem = sh.tmem;
 
+  // A tile's groups are fetched while the tile before is under way: a look into
+  // global memory takes microseconds when the memory is busy, and neither loads
+  // nor products may pause for it.
+  auto fetch = [&](uint32_t tile) {
+    return kSorted && lane < kTileGroups && tile < tiles ? o.tile_groups[tile % tiles_t * kTileGroups + lane]
+                                                         : Group{-1, ~0u, ~0u, 0};
+  };
+  auto put = [&](Group *list, const Group &mine) {
+    __syncwarp();
+    if (kSorted && lane < kTileGroups) list[lane] = mine;
+    __syncwarp();
+  };
+
+  // Both run as whole warps in step, one lane of which issues: what they count
+  // then stays in uniform registers, from which these instructions take their
+  // operands (a single lane alone needs 600 cycles a stage for moving them
+  // there, more than the products of 128 columns take).
   if (warp == 8) {
-    if (elect_one()) {
-      uint32_t at = 0, sent = 0;  // stage, and number of stages filled so far
-      bool ok = true;
-      auto take = [&](uint32_t expect) -> uint8_t * {  // the next stage, once it is free
-        if (sent >= p.stages) ok = mbar_wait(&sh.empty[at], (sent / p.stages - 1) & 1, gave_up);
-        if (!ok) return nullptr;
-        mbar_expect(&sh.full[at], expect);
-        return buf + (size_t)at * bytes;
-      };
-      auto next = [&] {
-        ++sent;
-        at = at + 1 == p.stages ? 0 : at + 1;
-      };
-      for (uint32_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
-        const int32_t v0 = (int32_t)(tile / tiles_t * kTileV);
-        const uint32_t tt = tile % tiles_t;
-        walk_tile(
-            a, o, kSorted, p.tile_t, groups, tt, chunks,
-            [&](uint32_t c) {
-              uint8_t *st = take(bytes);
-              if (!st) return false;
+    uint32_t at = 0, sent = 0;  // stage, and number of stages filled so far
+    bool ok = true;
+    auto open = [&] {  // the next stage, once it is free
+      if (sent >= p.stages) ok = mbar_wait(&sh.empty[at], (sent / p.stages - 1) & 1, gave_up);
+      ok = __all_sync(~0u, ok);
+      return ok;
+    };
+    auto next = [&] {
+      ++sent;
+      at = at + 1 == p.stages ? 0 : at + 1;
+    };
+    Group ahead = fetch(blockIdx.x);
+    for (uint32_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
+      put(sh.list[0], ahead);
+      ahead = fetch(tile + gridDim.x);
+      const int32_t v0 = (int32_t)(tile / tiles_t * kTileV);
+      const uint32_t tt = tile % tiles_t;
+      walk_tile(
+          a, p, o, kSorted, sh.list[0], tt, chunks,
+          [&](uint32_t c) {
+            if (!open()) return false;
+            uint8_t *st = buf + (size_t)at * bytes;
+            if (elect_one()) {
+              mbar_expect(&sh.full[at], bytes_w + p.tile_t * kTileD * 2);
               tma_load_2d(st, &map_w, &sh.full[at], (int32_t)(c * kTileD), v0);
               tma_load_2d(st + bytes_w, &map_h, &sh.full[at], (int32_t)(c * kTileD), (int32_t)(tt * p.tile_t));
-              next();
-              return true;
-            },
-            [&](int32_t adapter, uint32_t w0, uint32_t w, uint32_t r, uint32_t part, uint32_t parts) {
-              uint8_t *st = take(bytes_w + parts * w * kTileD * 2);
-              if (!st) return false;
-              tma_load_3d(st, &map_b, &sh.full[at], (int32_t)r, v0, adapter);
-              for (uint32_t x = 0; x < parts; ++x)
-                for (uint32_t i = 0; i < w; i += 16)
-                  tma_load_2d(st + bytes_w + (x * w + i) * kTileD * 2, &map_u, &sh.full[at], (int32_t)r,
-                              (int32_t)((part + x) * o.columns + w0 + i));
-              next();
-              return true;
-            });
-      }
-      // Copies must not land in a block that has ended: wait for the last fill
-      // of each stage (the products saw all of them full if nothing failed).
-      if (!ok)
-        for (uint32_t s = 0; s < p.stages && s < sent; ++s) {
-          const uint32_t fill = (sent - 1 - s) / p.stages;
-          for (uint32_t i = 0; i < kWaitTries && !mbar_try(&sh.full[s], fill & 1); ++i) {
-          }
-        }
+            }
+            next();
+            return true;
+          },
+          open,
+          [&](int32_t adapter, uint32_t w0, uint32_t w, uint32_t j, uint32_t offset) {
+            uint8_t *st = buf + (size_t)at * bytes + offset;
+            const uint32_t rows = kTileV * o.width * 2, cols = w * o.parts * o.width * 2;
+            if (elect_one()) {
+              mbar_expect_more(&sh.full[at], rows + cols);
+              tma_load_3d(st, &map_b, &sh.full[at], (int32_t)(j * o.width), v0, adapter);
+              bulk_load(st + rows, o.u + ((uint64_t)j * o.columns + w0) * o.parts * o.width * 2, cols, &sh.full[at]);
+            }
+            __syncwarp();
+          },
+          [&] {
+            if (elect_one()) mbar_arrive(&sh.full[at]);
+            next();
+          });
     }
+    // Copies must not land in a block that has ended: wait for the last fill
+    // of each stage (the products saw all of them full if nothing failed).
+    if (!ok)
+      for (uint32_t s = 0; s < p.stages && s < sent; ++s) {
+        const uint32_t fill = (sent - 1 - s) / p.stages;
+        for (uint32_t i = 0; i < kWaitTries && !mbar_try(&sh.full[s], fill & 1); ++i) {
+        }
+      }
   } else if (warp == 9) {
-    if (elect_one()) {
-      constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-      uint32_t at = 0, phase = 0, n = 0;
-      bool ok = true;
-      auto done = [&] {  // the stage is free when the products so far have ended
-        mma_commit(&sh.empty[at]);
-        if (++at == p.stages) at = 0, phase ^= 1;
-      };
-      for (uint32_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++n) {
-        const uint32_t b = n & 1, d = tmem + b * p.tmem_half, tt = tile % tiles_t, c0 = tt * p.tile_t;
-        const uint32_t shape = mma_shape(kBf16, kTileV, min(p.tile_t, (columns - c0 + 15) / 16 * 16));
-        if (n >= 2) ok = mbar_wait(&sh.acc_empty[b], (n / 2 - 1) & 1, gave_up);
-        if (!ok) break;
-        fence_after();
-        ok = walk_tile(
-            a, o, kSorted, p.tile_t, groups, tt, chunks,
-            [&](uint32_t c) {
-              if (!mbar_wait(&sh.full[at], phase, gave_up)) return false;
-              fence_after();
-              const uint64_t w = operand(buf + (size_t)at * bytes), h = operand(buf + (size_t)at * bytes + bytes_w);
+    constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+    uint32_t at = 0, phase = 0, n = 0;
+    bool ok = true;
+    const uint64_t first_w = operand(buf), first_h = operand(buf + bytes_w);
+    auto open = [&] {
+      ok = mbar_wait(&sh.full[at], phase, gave_up);
+      ok = __all_sync(~0u, ok);
+      fence_after();
+      return ok;
+    };
+    auto done = [&] {  // the stage is free when the products so far have ended
+      if (++at == p.stages) at = 0, phase ^= 1;
+    };
+    Group ahead = fetch(blockIdx.x);
+    for (uint32_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++n) {
+      put(sh.list[1], ahead);
+      ahead = fetch(tile + gridDim.x);
+      const uint32_t b = n & 1, d = tmem + b * p.tmem_half, tt = tile % tiles_t, c0 = tt * p.tile_t;
+      const uint32_t shape = mma_shape(kBf16, kTileV, min(p.tile_t, (columns - c0 + 15) / 16 * 16));
+      if (n >= 2) ok = __all_sync(~0u, mbar_wait(&sh.acc_empty[b], (n / 2 - 1) & 1, gave_up));
+      if (!ok) break;
+      fence_after();
+      walk_tile(
+          a, p, o, kSorted, sh.list[1], tt, chunks,
+          [&](uint32_t c) {
+            if (!open()) return false;
+            const uint64_t w = first_w + (at * bytes >> 4), h = first_h + (at * bytes >> 4);
+            if (elect_one()) {
 #pragma unroll
               for (int k = 0; k < kTileD / 16; ++k) mma_f16(d, w + 2 * k, h + 2 * k, shape, c > 0 || k > 0);
-              done();
-              return true;
-            },
-            [&](int32_t, uint32_t w0, uint32_t w, uint32_t r, uint32_t, uint32_t parts) {
-              if (!mbar_wait(&sh.full[at], phase, gave_up)) return false;
-              fence_after();
-              const uint8_t *st = buf + (size_t)at * bytes;
-              const uint64_t bw = operand(st);
-              const uint32_t steps = (min(a.rank - r, (uint32_t)kTileD) + 15) / 16, narrow = mma_shape(kBf16, kTileV, w);
-              for (uint32_t x = 0; x < parts; ++x) {
-                const uint64_t uw = operand(st + bytes_w + x * w * kTileD * 2);
+              mma_commit(&sh.empty[at]);
+            }
+            done();
+            return true;
+          },
+          open,
+          [&](int32_t, uint32_t w0, uint32_t w, uint32_t j, uint32_t offset) {
+            const uint32_t row = o.width * 2, rows = kTileV * row;
+            const uint8_t *st = buf + (size_t)at * bytes + offset;
+            const uint64_t bw = operand(st, row, 8 * row);
+            const uint32_t steps = (min(a.rank - j * o.width, o.width) + 15) / 16;
+            const uint32_t narrow = mma_shape(kBf16, kTileV, w);
+            if (elect_one())
+              for (uint32_t x = 0; x < o.parts; ++x) {
+                const uint64_t uw = operand(st + rows + x * 8 * row, row, o.parts * 8 * row);
                 for (uint32_t k = 0; k < steps; ++k) mma_f16(d + (w0 - c0), bw + 2 * k, uw + 2 * k, narrow, true);
               }
-              done();
-              return true;
-            });
-        if (ok) mma_commit(&sh.acc_full[b]);
-      }
+            __syncwarp();
+          },
+          [&] {
+            if (elect_one()) mma_commit(&sh.empty[at]);
+            done();
+          });
+      if (ok && elect_one()) mma_commit(&sh.acc_full[b]);
     }
   } else {
     // Warps w and w + 4 read the same quarter of tensor memory (its lanes
@@ -410,7 +533,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         int32_t token = -1, id = -1;
         if (c0 + (lane & 15) < count) {
           token = kSorted ? o.col_token[mine] : (int32_t)mine;
-          if (!kSorted && u) id = a.adapter_ids[mine / a.num_outpos];
+          if (!kSorted && delta) id = a.adapter_ids[mine / a.num_outpos];
         }
         uint32_t acc[16];
         if (ok) {
@@ -420,44 +543,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int e = 0; e < 16; ++e) acc[e] = 0x7FC00000;
         }
-        if (!kSorted && u) {
-          // The low-rank part in 32 bits; all 16 rows of B on their way before
-          // the first is used.
-          const uint32_t any = __ballot_sync(~0u, (uint32_t)id < a.num_adapters) & 0xFFFF;
-          const uint32_t wrong = __ballot_sync(~0u, (uint32_t)id >= a.num_adapters && id != -1) & 0xFFFF;
-          const T *base = static_cast<const T *>(a.lora_b) + (uint64_t)(live ? v : 0) * a.rank;
-          for (uint32_t r = 0; any && r < a.rank; r += 8) {
-            uint4 w[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int32_t at = __shfl_sync(~0u, id, e);
-              const int32_t before = e ? __shfl_sync(~0u, id, e ? e - 1 : 0) : -1;
-              if (any >> e & 1) {
-                if (e && at == before)
-                  w[e] = w[e ? e - 1 : 0];
-                else
-                  w[e] = __ldg(reinterpret_cast<const uint4 *>(base + (uint64_t)at * a.vocab * a.rank + r));
-              } else {
-                w[e] = make_uint4(0, 0, 0, 0);
-              }
-            }
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              if (any >> e & 1) {
-                float y[8];
-                unpack8<T>(w[e], y);
-                const float4 *x = reinterpret_cast<const float4 *>(u + (uint64_t)(t0 + c0 + e) * a.rank + r);
-                const float4 x0 = __ldg(x), x1 = __ldg(x + 1);
-                float s = __uint_as_float(acc[e]);
-                s = fmaf(x0.x, y[0], s), s = fmaf(x0.y, y[1], s), s = fmaf(x0.z, y[2], s), s = fmaf(x0.w, y[3], s);
-                s = fmaf(x1.x, y[4], s), s = fmaf(x1.y, y[5], s), s = fmaf(x1.z, y[6], s), s = fmaf(x1.w, y[7], s);
-                acc[e] = __float_as_uint(s);
-              }
-            }
-          }
+        if (!kSorted && delta) {
+          const uint32_t any = __ballot_sync(~0u, (uint32_t)id < a.num_adapters);
+          const uint32_t wrong = __ballot_sync(~0u, (uint32_t)id >= a.num_adapters && id != -1);
+          float more[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            if (wrong >> e & 1) acc[e] = 0x7FC00000;
+            more[e] = live && (any >> e & 1) ? __ldg(&delta[(uint64_t)(t0 + c0 + e) * a.vocab + v]) : 0.0f;
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            acc[e] = wrong >> e & 1 ? 0x7FC00000 : __float_as_uint(__uint_as_float(acc[e]) + more[e]);
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -498,17 +593,21 @@ EncodeFn encode_fn() {
   return fn;
 }
 
-// `layers` arrays of rows of `inner` 16-bit values, loaded as boxes of 64
-// values by `box` rows with the 128-byte swizzle; what lies outside reads as 0.
-CUtensorMap make_map(const void *base, bool bf16, uint64_t inner, uint64_t rows, uint64_t layers, uint32_t box,
-                     const char *what) {
+// `layers` arrays of rows of `inner` 16-bit values, loaded as boxes of `width`
+// (16, 32 or 64) values by `box` rows, swizzled over that width; what lies
+// outside reads as 0.
+CUtensorMap make_map(const void *base, bool bf16, uint64_t inner, uint64_t rows, uint64_t layers, uint32_t width,
+                     uint32_t box, const char *what) {
   CUtensorMap m;
   const cuuint64_t dims[3] = {inner, rows, layers}, strides[2] = {inner * 2, inner * rows * 2};
-  const cuuint32_t tile[3] = {(cuuint32_t)kTileD, box, 1}, step[3] = {1, 1, 1};
+  const cuuint32_t tile[3] = {width, box, 1}, step[3] = {1, 1, 1};
+  const CUtensorMapSwizzle swizzle = width == 64   ? CU_TENSOR_MAP_SWIZZLE_128B
+                                     : width == 32 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                   : CU_TENSOR_MAP_SWIZZLE_32B;
   const CUresult rc =
       encode_fn()(&m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, layers ? 3 : 2,
                   const_cast<void *>(base), dims, strides, tile, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (rc != CUDA_SUCCESS)
     throw CudaError(std::string("CUDA error: cuTensorMapEncodeTiled refused ") + what + " (" + std::to_string((int)rc) + ")");
   return m;
@@ -533,7 +632,8 @@ void check_adapter(const ft_adapter_args &a) {
   if (a.num_adapters > kMaxAdapters) throw InvalidArgument("adapter_logits: at most 65536 adapters");
   // Token and vocabulary coordinates of a tile are 32-bit.
   if ((uint64_t)a.n * a.num_outpos > 0x3FFFFF || a.vocab > 0x7FFFFF00u || a.dim > 0xFFFFFF ||
-      (uint64_t)(a.vocab / kTileV + 1) * ((uint64_t)a.n * a.num_outpos / 16 + 1) > 0x7FFFFFFF)
+      (uint64_t)(a.vocab / kTileV + 1) * ((uint64_t)a.n * a.num_outpos / 16 + 1) > 0x7FFFFFFF ||
+      (uint64_t)(a.vocab / 256 + 1) * a.n > 0x7FFFFFFF)
     throw InvalidArgument("adapter_logits: too many tokens or too large a vocabulary");
 }
 
@@ -542,14 +642,14 @@ uint64_t align256(uint64_t x) { return (x + 255) & ~(uint64_t)255; }
 // Which form a call takes and where its workspace's parts lie.
 struct Layout {
   bool sorted = false;
-  uint32_t tokens = 0, columns = 0, parts = 0;
-  uint64_t head = 0, groups = 0, tile_first = 0, req_col = 0, col_token = 0, hidden = 0, u = 0, end = 0;
+  uint32_t tokens = 0, columns = 0, parts = 0, width = 0;
+  uint64_t delta = 0, head = 0, groups = 0, tile_first = 0, tile_groups = 0, req_col = 0, col_token = 0, hidden = 0, u = 0, end = 0;
 };
 
 Layout layout_of(const ft_adapter_args &a) {
   Layout l;
   l.tokens = l.columns = a.n * a.num_outpos;
-  if (!a.num_adapters) return l;
+  if (!a.num_adapters || l.tokens == 0) return l;
   // Padding a group to a multiple of 16 columns adds at most 16 - gcd(L, 16).
   const uint64_t groups = std::min<uint64_t>(a.n, (uint64_t)a.num_adapters + 1);
   uint32_t step = 1;
@@ -557,10 +657,12 @@ Layout layout_of(const ft_adapter_args &a) {
   const uint64_t most = ((uint64_t)l.tokens + groups * (16 - step) + 15) / 16 * 16;
   l.sorted = a.n <= kMaxSortRequests && most <= 2 * (uint64_t)l.tokens;
   if (!l.sorted) {
-    l.end = align256((uint64_t)l.tokens * a.rank * 4);
+    l.delta = align256((uint64_t)l.tokens * a.rank * 4);
+    l.end = l.delta + align256((uint64_t)l.tokens * a.vocab * 4);
     return l;
   }
   l.columns = (uint32_t)most;
+  l.width = a.rank <= 16 ? 16 : a.rank <= 32 ? 32 : 64;
   l.parts = a.dtype == FT_DTYPE_BF16 && a.out_dtype == FT_DTYPE_F32 ? 3 : 2;
   uint64_t at = 256;
   auto place = [&](uint64_t bytes) {
@@ -570,10 +672,11 @@ Layout layout_of(const ft_adapter_args &a) {
   };
   l.groups = place(sizeof(Group) * groups);
   l.tile_first = place(4 * (most / 16 + 1));
+  l.tile_groups = place(sizeof(Group) * kTileGroups * (most / plan_logits(a, l.columns, l.parts).tile_t + 1));
   l.req_col = place(4ull * a.n);
   l.col_token = place(4 * most);
   l.hidden = place(most * a.dim * 2);
-  l.u = place(l.parts * most * a.rank * 2);
+  l.u = place((uint64_t)((a.rank + l.width - 1) / l.width) * most * l.parts * l.width * 2);
   l.end = at;
   return l;
 }
@@ -600,24 +703,22 @@ void adapter_logits_device(const ft_adapter_args &a, void *ws, uint64_t ws_bytes
   const Layout l = layout_of(a);
   if (ws_bytes < l.end || (l.end && (!ws || (reinterpret_cast<uintptr_t>(ws) & 255))))
     throw InvalidArgument("adapter_logits: needs a 256-byte aligned workspace of " + std::to_string(l.end) + " bytes");
-  const LogitsPlan p = plan_logits(a, l.columns);
+  const LogitsPlan p = plan_logits(a, l.columns, l.parts);
   uint8_t *w = static_cast<uint8_t *>(ws);
   float *u = a.num_adapters && !l.sorted ? reinterpret_cast<float *>(w) : nullptr;
+  float *delta = u ? reinterpret_cast<float *>(w + l.delta) : nullptr;
   Sorted o{};
   if (l.sorted)
     o = Sorted{reinterpret_cast<uint32_t *>(w + l.head),    reinterpret_cast<Group *>(w + l.groups),
-               reinterpret_cast<uint32_t *>(w + l.tile_first), reinterpret_cast<uint32_t *>(w + l.req_col),
+               reinterpret_cast<uint32_t *>(w + l.tile_first),
+               reinterpret_cast<Group *>(w + l.tile_groups), reinterpret_cast<uint32_t *>(w + l.req_col),
                reinterpret_cast<int32_t *>(w + l.col_token), w + l.hidden,
-               w + l.u,                                      l.columns,
-               l.parts};
+               w + l.u, l.columns, l.parts, l.width};
   const bool bf16 = a.dtype == FT_DTYPE_BF16;
-  const CUtensorMap map_w = make_map(a.weight, bf16, a.dim, a.vocab, 0, kTileV, "weight");
-  const CUtensorMap map_h = make_map(l.sorted ? o.hidden : a.hidden, bf16, a.dim, l.columns, 0, p.tile_t, "hidden");
-  CUtensorMap map_b = map_w, map_u = map_w;
-  if (l.sorted) {
-    map_b = make_map(a.lora_b, bf16, a.rank, a.vocab, a.num_adapters, kTileV, "lora_b");
-    map_u = make_map(o.u, bf16, a.rank, (uint64_t)l.parts * l.columns, 0, 16, "the low-rank values");
-  }
+  const CUtensorMap map_w = make_map(a.weight, bf16, a.dim, a.vocab, 0, kTileD, kTileV, "weight");
+  const CUtensorMap map_h = make_map(l.sorted ? o.hidden : a.hidden, bf16, a.dim, l.columns, 0, kTileD, p.tile_t, "hidden");
+  CUtensorMap map_b = map_w;
+  if (l.sorted) map_b = make_map(a.lora_b, bf16, a.rank, a.vocab, a.num_adapters, l.width, kTileV, "lora_b");
   const size_t smem = logits_smem(p);
   const unsigned grid = std::min<unsigned>(p.tiles_t * p.tiles_v, (unsigned)sm_count());
   const unsigned shrink = a.n * ((a.num_outpos + kShrinkTokens - 1) / kShrinkTokens);
@@ -632,7 +733,7 @@ void adapter_logits_device(const ft_adapter_args &a, void *ws, uint64_t ws_bytes
   }
   auto launch = [&](auto *kernel) {
     CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    kernel<<<grid, kThreads, smem, stream>>>(map_w, map_h, map_b, map_u, a, p, u, o);
+    kernel<<<grid, kThreads, smem, stream>>>(map_w, map_h, map_b, a, p, delta, o);
     CUDA_TRY(cudaGetLastError());
   };
   auto run = [&](auto *t) {
@@ -642,6 +743,11 @@ void adapter_logits_device(const ft_adapter_args &a, void *ws, uint64_t ws_bytes
     else if (u)
       shrink_kernel<T, false><<<shrink, 256, 0, stream>>>(a, u, o);
     CUDA_TRY(cudaGetLastError());
+    if (u) {
+      const unsigned blocks = a.n * ((a.vocab + kExpandThreads - 1) / kExpandThreads);
+      expand_kernel<T><<<blocks, kExpandThreads, 0, stream>>>(a, u, delta);
+      CUDA_TRY(cudaGetLastError());
+    }
     if (l.sorted)
       a.out_dtype == FT_DTYPE_F32 ? launch(logits_kernel<T, float, true>) : launch(logits_kernel<T, T, true>);
     else

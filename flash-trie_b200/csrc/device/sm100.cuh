@@ -27,6 +27,10 @@ __device__ __forceinline__ void mbar_init_fence() { asm volatile("fence.mbarrier
 __device__ __forceinline__ void mbar_expect(uint64_t *bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
 }
+// More bytes for the phase under way, without an arrival.
+__device__ __forceinline__ void mbar_expect_more(uint64_t *bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
@@ -76,6 +80,14 @@ __device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, u
       : "memory");
 }
 
+// A run of bytes: both addresses and the size are multiples of 16.
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_addr(dst)),
+               "l"(src), "r"(bytes), "r"(smem_addr(bar))
+               : "memory");
+}
+
 __device__ __forceinline__ void tmem_alloc(uint32_t *at, uint32_t columns) {
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(at)), "r"(columns)
                : "memory");
@@ -87,11 +99,17 @@ __device__ __forceinline__ void tmem_free(uint32_t base, uint32_t columns) {
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// Shared-memory operand of rows of 128 bytes (64 16-bit values along the inner
-// dimension), 128-byte swizzle, groups of 8 rows 1024 bytes apart.
-__device__ __forceinline__ uint64_t operand(const void *smem) {
-  return (uint64_t)((smem_addr(smem) & 0x3FFFF) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+// Shared-memory operand whose rows hold 128, 64 or 32 bytes along the inner
+// dimension, swizzled over that width; groups of 8 rows are `apart` bytes apart.
+__device__ __forceinline__ uint64_t operand(const void *smem, uint32_t row_bytes = 128, uint32_t apart = 1024) {
+  const uint64_t layout = row_bytes == 128 ? 2 : row_bytes == 64 ? 4 : 6;
+  return (uint64_t)((smem_addr(smem) & 0x3FFFF) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(apart >> 4) << 32) |
+         ((uint64_t)1 << 46) | (layout << 61);
+}
+// The same swizzle for a byte offset from the start of a group of 8 rows: the
+// 16-byte piece is exchanged by the number of its 128 bytes.
+__device__ __forceinline__ uint32_t swizzled(uint32_t offset, uint32_t row_bytes) {
+  return offset ^ ((offset >> 7 & (row_bytes / 16 - 1)) << 4);
 }
 // f32 accumulator, both operands bf16 (or both f16), inner dimension contiguous.
 __host__ __device__ constexpr uint32_t mma_shape(bool bf16, uint32_t m, uint32_t n) {
