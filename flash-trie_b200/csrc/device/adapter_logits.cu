@@ -33,7 +33,7 @@ namespace {
 constexpr uint32_t kMaxRank = 256;
 constexpr uint32_t kMaxAdapters = 65536;
 
-constexpr int kTileV = 128;   // vocabulary entries of a tile (rows of the product)
+constexpr int kTileV = 128;   // vocabulary entries of one product's rows; a tile has one or two such halves
 constexpr int kTileD = 64;    // inner dimension of a stage: 128-byte rows
 constexpr int kMaxTileT = 256;
 constexpr int kMaxStages = 12;
@@ -291,32 +291,40 @@ struct LogitsPlan {
   uint32_t columns;    // tokens, or the sorted form's upper bound
   uint32_t tile_t;     // columns of a tile, a multiple of 16
   uint32_t tiles_t;
+  uint32_t halves;     // 128 vocabulary entries each
   uint32_t tiles_v;
-  uint32_t slot_t;     // rows that a stage has for them
+  uint32_t stage;      // bytes
   uint32_t stages;
-  uint32_t tmem_half;  // columns of one of the two accumulators
+  uint32_t acc;        // tensor memory columns of one accumulator
+  // Bytes that a group of columns takes in a stage: for its adapter's rows, and
+  // for its low-rank values per column; and how many columns fit.
+  uint32_t group_rows, group_column, group_most;
 };
 
 struct alignas(8) LogitsShared {
   uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
-  Group list[2][kTileGroups];  // of the tile that loads and products are at
   uint32_t tmem, gave_up;
 };
 
-LogitsPlan plan_logits(const ft_adapter_args &a, uint32_t columns, uint32_t parts) {
+LogitsPlan plan_logits(const ft_adapter_args &a, uint32_t columns, uint32_t parts, uint32_t width) {
   LogitsPlan p;
   p.columns = columns;
   p.tiles_t = (columns + kMaxTileT - 1) / kMaxTileT;
   p.tile_t = ((columns + p.tiles_t - 1) / p.tiles_t + 15) / 16 * 16;
-  p.tiles_v = (a.vocab + kTileV - 1) / kTileV;
-  p.slot_t = std::max(p.tile_t, 16 * parts);
-  const uint32_t stage = (kTileV + p.slot_t) * kTileD * 2;
-  p.stages = std::min<uint32_t>(kMaxStages, (225 * 1024) / stage);
-  p.tmem_half = 32;
-  while (p.tmem_half < p.tile_t) p.tmem_half *= 2;
+  p.acc = 32;
+  while (p.acc < p.tile_t) p.acc *= 2;
+  // Two halves share the tokens' part of a stage, where two accumulators of
+  // each fit into the 512 columns and there are tiles enough for all SMs.
+  p.halves = p.acc <= 128 && a.vocab >= 148 * 4 * kTileV ? 2 : 1;
+  p.tiles_v = (a.vocab + p.halves * kTileV - 1) / (p.halves * kTileV);
+  p.stage = (p.halves * kTileV + std::max(p.tile_t, 16 * parts)) * kTileD * 2;
+  p.stages = std::min<uint32_t>(kMaxStages, (225 * 1024) / p.stage);
+  p.group_rows = p.halves * kTileV * width * 2;
+  p.group_column = parts * width * 2;
+  p.group_most = parts ? (p.stage - p.group_rows) / p.group_column / 16 * 16 : 0;
   return p;
 }
-size_t logits_smem(const LogitsPlan &p) { return 1024 + (size_t)p.stages * (kTileV + p.slot_t) * kTileD * 2; }
+size_t logits_smem(const LogitsPlan &p) { return 1024 + (size_t)p.stages * p.stage; }
 
 // The stages of a tile in the order that loads and products both take them:
 // the shared projection's, then those of each group that has columns in it.
@@ -324,30 +332,31 @@ size_t logits_smem(const LogitsPlan &p) { return 1024 + (size_t)p.stages * (kTil
 // fit: g(adapter, first column, width, low-rank slice, offset in the stage),
 // with open() before the first of a stage and close() after the last. A
 // callback that returns false ends the walk.
+// `mine`: the tile's groups, one a lane. The whole warp takes part.
 template <typename F, typename Open, typename G, typename Close>
 __device__ __forceinline__ bool walk_tile(const ft_adapter_args &a, const LogitsPlan &p, const Sorted &o, bool sorted,
-                                          const Group *list, uint32_t tt, uint32_t chunks, F &&f, Open &&open, G &&g,
+                                          const Group &mine, uint32_t c0, uint32_t chunks, F &&f, Open &&open, G &&g,
                                           Close &&close) {
   for (uint32_t c = 0; c < chunks; ++c)
     if (!f(c)) return false;
   if (!sorted) return true;
-  const uint32_t c0 = tt * p.tile_t, c1 = c0 + p.tile_t, room = (kTileV + p.slot_t) * kTileD * 2;
-  const uint32_t fixed = kTileV * o.width * 2, each = o.parts * o.width * 2;  // bytes of B, and of u per column
-  const uint32_t most = (room - fixed) / each / 16 * 16;
+  const uint32_t c1 = c0 + p.tile_t;
   uint32_t used = 0;
-  for (uint32_t i = 0; list[i].col0 < c1; ++i) {
-    const Group q = list[i];
-    if (q.adapter < 0) continue;
-    const uint32_t end = min(q.col1, c1);
-    for (uint32_t w0 = max(q.col0, c0); w0 < end; w0 += most)
+  for (uint32_t i = 0;; ++i) {
+    const uint32_t col0 = __shfl_sync(~0u, mine.col0, i), col1 = __shfl_sync(~0u, mine.col1, i);
+    const int32_t adapter = __shfl_sync(~0u, mine.adapter, i);
+    if (col0 >= c1) break;  // the list ends with such a one
+    if (adapter < 0) continue;
+    const uint32_t end = min(col1, c1);
+    for (uint32_t w0 = max(col0, c0); w0 < end; w0 += p.group_most)
       for (uint32_t j = 0; j * o.width < a.rank; ++j) {
-        const uint32_t w = min(most, end - w0), need = fixed + w * each;
-        if (used && used + need > room) {
+        const uint32_t w = min(p.group_most, end - w0), need = p.group_rows + w * p.group_column;
+        if (used && used + need > p.stage) {
           close();
           used = 0;
         }
         if (!used && !open()) return false;
-        g(q.adapter, w0, w, j, used);
+        g(adapter, w0, w, j, used);
         used += need;
       }
   }
@@ -366,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t *buf = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   __shared__ LogitsShared sh;
   const uint32_t warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const uint32_t bytes_w = kTileV * kTileD * 2, bytes = bytes_w + p.slot_t * kTileD * 2;
+  const uint32_t bytes_w = p.halves * kTileV * kTileD * 2, bytes = p.stage;
   const uint32_t columns = kSorted ? o.head[1] : p.columns;
   const uint32_t tiles_t = (columns + p.tile_t - 1) / p.tile_t;
   const uint32_t tiles = tiles_t * p.tiles_v, chunks = (a.dim + kTileD - 1) / kTileD;
@@ -379,23 +388,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_map(&map_w);
     prefetch_map(&map_h);
   }
-  if (warp == 9) tmem_alloc(&sh.tmem, 2 * p.tmem_half);
+  if (warp == 9) tmem_alloc(&sh.tmem, 2 * p.halves * p.acc);
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = sh.tmem;
 
-  // A tile's groups are fetched while the tile before is under way: a look into
-  // global memory takes microseconds when the memory is busy, and neither loads
-  // nor products may pause for it.
+  // A tile's groups, one a lane, are fetched while the tile before is under
+  // way: a look into global memory takes microseconds when the memory is busy,
+  // and neither loads nor products may pause for it.
   auto fetch = [&](uint32_t tile) {
     return kSorted && lane < kTileGroups && tile < tiles ? o.tile_groups[tile % tiles_t * kTileGroups + lane]
                                                          : Group{-1, ~0u, ~0u, 0};
-  };
-  auto put = [&](Group *list, const Group &mine) {
-    __syncwarp();
-    if (kSorted && lane < kTileGroups) list[lane] = mine;
-    __syncwarp();
   };
 
   // Both run as whole warps in step, one lane of which issues: what they count
@@ -416,19 +420,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     Group ahead = fetch(blockIdx.x);
     for (uint32_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
-      put(sh.list[0], ahead);
+      const Group mine = ahead;
       ahead = fetch(tile + gridDim.x);
-      const int32_t v0 = (int32_t)(tile / tiles_t * kTileV);
-      const uint32_t tt = tile % tiles_t;
+      const int32_t v0 = (int32_t)(tile / tiles_t * p.halves * kTileV), t0 = (int32_t)(tile % tiles_t * p.tile_t);
       walk_tile(
-          a, p, o, kSorted, sh.list[0], tt, chunks,
+          a, p, o, kSorted, mine, (uint32_t)t0, chunks,
           [&](uint32_t c) {
             if (!open()) return false;
             uint8_t *st = buf + (size_t)at * bytes;
             if (elect_one()) {
               mbar_expect(&sh.full[at], bytes_w + p.tile_t * kTileD * 2);
               tma_load_2d(st, &map_w, &sh.full[at], (int32_t)(c * kTileD), v0);
-              tma_load_2d(st + bytes_w, &map_h, &sh.full[at], (int32_t)(c * kTileD), (int32_t)(tt * p.tile_t));
+              tma_load_2d(st + bytes_w, &map_h, &sh.full[at], (int32_t)(c * kTileD), t0);
             }
             next();
             return true;
@@ -436,13 +439,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           open,
           [&](int32_t adapter, uint32_t w0, uint32_t w, uint32_t j, uint32_t offset) {
             uint8_t *st = buf + (size_t)at * bytes + offset;
-            const uint32_t rows = kTileV * o.width * 2, cols = w * o.parts * o.width * 2;
             if (elect_one()) {
-              mbar_expect_more(&sh.full[at], rows + cols);
+              mbar_expect_more(&sh.full[at], p.group_rows + w * p.group_column);
               tma_load_3d(st, &map_b, &sh.full[at], (int32_t)(j * o.width), v0, adapter);
-              bulk_load(st + rows, o.u + ((uint64_t)j * o.columns + w0) * o.parts * o.width * 2, cols, &sh.full[at]);
+              bulk_load(st + p.group_rows, o.u + ((uint64_t)j * o.columns + w0) * p.group_column, w * p.group_column,
+                        &sh.full[at]);
             }
-            __syncwarp();
           },
           [&] {
             if (elect_one()) mbar_arrive(&sh.full[at]);
@@ -473,21 +475,26 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     Group ahead = fetch(blockIdx.x);
     for (uint32_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++n) {
-      put(sh.list[1], ahead);
+      const Group mine = ahead;
       ahead = fetch(tile + gridDim.x);
-      const uint32_t b = n & 1, d = tmem + b * p.tmem_half, tt = tile % tiles_t, c0 = tt * p.tile_t;
+      const uint32_t b = n & 1, d = tmem + b * p.halves * p.acc, c0 = tile % tiles_t * p.tile_t;
       const uint32_t shape = mma_shape(kBf16, kTileV, min(p.tile_t, (columns - c0 + 15) / 16 * 16));
       if (n >= 2) ok = __all_sync(~0u, mbar_wait(&sh.acc_empty[b], (n / 2 - 1) & 1, gave_up));
       if (!ok) break;
       fence_after();
       walk_tile(
-          a, p, o, kSorted, sh.list[1], tt, chunks,
+          a, p, o, kSorted, mine, c0, chunks,
           [&](uint32_t c) {
             if (!open()) return false;
             const uint64_t w = first_w + (at * bytes >> 4), h = first_h + (at * bytes >> 4);
             if (elect_one()) {
 #pragma unroll
               for (int k = 0; k < kTileD / 16; ++k) mma_f16(d, w + 2 * k, h + 2 * k, shape, c > 0 || k > 0);
+              if (p.halves == 2) {
+#pragma unroll
+                for (int k = 0; k < kTileD / 16; ++k)
+                  mma_f16(d + p.acc, w + (kTileV * kTileD * 2 >> 4) + 2 * k, h + 2 * k, shape, c > 0 || k > 0);
+              }
               mma_commit(&sh.empty[at]);
             }
             done();
@@ -495,17 +502,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           },
           open,
           [&](int32_t, uint32_t w0, uint32_t w, uint32_t j, uint32_t offset) {
-            const uint32_t row = o.width * 2, rows = kTileV * row;
+            const uint32_t row = o.width * 2;
             const uint8_t *st = buf + (size_t)at * bytes + offset;
-            const uint64_t bw = operand(st, row, 8 * row);
+            const uint64_t bw = operand(st, row, 8 * row), uw = operand(st + p.group_rows, row, o.parts * 8 * row);
             const uint32_t steps = (min(a.rank - j * o.width, o.width) + 15) / 16;
-            const uint32_t narrow = mma_shape(kBf16, kTileV, w);
+            const uint32_t narrow = mma_shape(kBf16, kTileV, w), to = d + (w0 - c0);
             if (elect_one())
-              for (uint32_t x = 0; x < o.parts; ++x) {
-                const uint64_t uw = operand(st + rows + x * 8 * row, row, o.parts * 8 * row);
-                for (uint32_t k = 0; k < steps; ++k) mma_f16(d + (w0 - c0), bw + 2 * k, uw + 2 * k, narrow, true);
-              }
-            __syncwarp();
+              for (uint32_t half = 0; half < p.halves; ++half)
+                for (uint32_t x = 0; x < o.parts; ++x)
+                  for (uint32_t k = 0; k < steps; ++k)
+                    mma_f16(to + half * p.acc, bw + (half * kTileV * row >> 4) + 2 * k, uw + (x * 8 * row >> 4) + 2 * k,
+                            narrow, true);
           },
           [&] {
             if (elect_one()) mma_commit(&sh.empty[at]);
@@ -515,19 +522,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // Warps w and w + 4 read the same quarter of tensor memory (its lanes
-    // 32 (w % 4) on); they take alternate blocks of 16 columns.
+    // 32 (w % 4) on); they take one half of the vocabulary entries each, or
+    // alternate blocks of 16 columns.
     uint32_t n = 0;
     bool ok = true;
-    const uint32_t row = (warp & 3) * 32 + lane;
+    const uint32_t half = p.halves == 2 ? warp >> 2 : 0, row = half * kTileV + (warp & 3) * 32 + lane;
     for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
       const uint32_t b = n & 1, t0 = tile % tiles_t * p.tile_t;
-      const uint32_t v = tile / tiles_t * kTileV + row;
+      const uint32_t v = tile / tiles_t * p.halves * kTileV + row;
       const bool live = v < a.vocab;
       const uint32_t count = min(p.tile_t, columns - t0);
       if (ok) ok = mbar_wait(&sh.acc_full[b], (n / 2) & 1, gave_up);
       ok = __all_sync(~0u, ok);
       if (ok) fence_after();
-      for (uint32_t c0 = (warp >> 2) * 16; c0 < count; c0 += 32) {
+      for (uint32_t c0 = p.halves == 2 ? 0 : (warp >> 2) * 16; c0 < count; c0 += p.halves == 2 ? 16 : 32) {
         // Lane e (and e + 16) looks up what column c0 + e is.
         const uint32_t mine = t0 + c0 + (lane & 15);
         int32_t token = -1, id = -1;
@@ -537,7 +545,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         uint32_t acc[16];
         if (ok) {
-          tmem_load16(tmem + b * p.tmem_half + c0 + ((warp & 3) << 21), acc);
+          tmem_load16(tmem + (b * p.halves + half) * p.acc + c0 + ((warp & 3) << 21), acc);
         } else {
           // A wait ran out: no result is better than a wrong one.
 #pragma unroll
@@ -575,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_before();
   __syncthreads();
   fence_after();
-  if (warp == 9) tmem_free(tmem, 2 * p.tmem_half);
+  if (warp == 9) tmem_free(tmem, 2 * p.halves * p.acc);
 }
 
 using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
@@ -672,7 +680,7 @@ Layout layout_of(const ft_adapter_args &a) {
   };
   l.groups = place(sizeof(Group) * groups);
   l.tile_first = place(4 * (most / 16 + 1));
-  l.tile_groups = place(sizeof(Group) * kTileGroups * (most / plan_logits(a, l.columns, l.parts).tile_t + 1));
+  l.tile_groups = place(sizeof(Group) * kTileGroups * (most / plan_logits(a, l.columns, l.parts, l.width).tile_t + 1));
   l.req_col = place(4ull * a.n);
   l.col_token = place(4 * most);
   l.hidden = place(most * a.dim * 2);
@@ -703,7 +711,7 @@ void adapter_logits_device(const ft_adapter_args &a, void *ws, uint64_t ws_bytes
   const Layout l = layout_of(a);
   if (ws_bytes < l.end || (l.end && (!ws || (reinterpret_cast<uintptr_t>(ws) & 255))))
     throw InvalidArgument("adapter_logits: needs a 256-byte aligned workspace of " + std::to_string(l.end) + " bytes");
-  const LogitsPlan p = plan_logits(a, l.columns, l.parts);
+  const LogitsPlan p = plan_logits(a, l.columns, l.parts, l.width);
   uint8_t *w = static_cast<uint8_t *>(ws);
   float *u = a.num_adapters && !l.sorted ? reinterpret_cast<float *>(w) : nullptr;
   float *delta = u ? reinterpret_cast<float *>(w + l.delta) : nullptr;
@@ -715,10 +723,10 @@ void adapter_logits_device(const ft_adapter_args &a, void *ws, uint64_t ws_bytes
                reinterpret_cast<int32_t *>(w + l.col_token), w + l.hidden,
                w + l.u, l.columns, l.parts, l.width};
   const bool bf16 = a.dtype == FT_DTYPE_BF16;
-  const CUtensorMap map_w = make_map(a.weight, bf16, a.dim, a.vocab, 0, kTileD, kTileV, "weight");
+  const CUtensorMap map_w = make_map(a.weight, bf16, a.dim, a.vocab, 0, kTileD, p.halves * kTileV, "weight");
   const CUtensorMap map_h = make_map(l.sorted ? o.hidden : a.hidden, bf16, a.dim, l.columns, 0, kTileD, p.tile_t, "hidden");
   CUtensorMap map_b = map_w;
-  if (l.sorted) map_b = make_map(a.lora_b, bf16, a.rank, a.vocab, a.num_adapters, l.width, kTileV, "lora_b");
+  if (l.sorted) map_b = make_map(a.lora_b, bf16, a.rank, a.vocab, a.num_adapters, l.width, p.halves * kTileV, "lora_b");
   const size_t smem = logits_smem(p);
   const unsigned grid = std::min<unsigned>(p.tiles_t * p.tiles_v, (unsigned)sm_count());
   const unsigned shrink = a.n * ((a.num_outpos + kShrinkTokens - 1) / kShrinkTokens);
