@@ -37,9 +37,11 @@ constexpr int kTileV = 128;   // vocabulary entries of one product's rows; a til
 constexpr int kTileD = 64;    // inner dimension of a stage: 128-byte rows
 constexpr int kMaxTileT = 256;
 constexpr int kMaxStages = 12;
-constexpr int kEpilogue = 256;            // threads of warps 0-7
-constexpr int kThreads = kEpilogue + 64;  // warp 8: loads, warp 9: products
+constexpr int kEpilogue = 512;            // threads of warps 0-15; with half of them the stores take half as long again
+constexpr int kThreads = kEpilogue + 64;  // warp 16: loads, warp 17: products
+constexpr uint32_t kLoadWarp = kEpilogue / 32, kProductWarp = kLoadWarp + 1;
 constexpr uint32_t kMaxSortRequests = 8192;
+static_assert(kEpilogue >= kMaxTileT, "a thread of the epilogue looks up each column");
 
 template <typename T>
 __device__ __forceinline__ void unpack8(uint4 q, float (&v)[8]) {
@@ -48,6 +50,16 @@ __device__ __forceinline__ void unpack8(uint4 q, float (&v)[8]) {
 
 // A group has at least 16 columns, so that a tile has 16 groups at most.
 constexpr uint32_t kTileGroups = kMaxTileT / 16 + 1;
+
+__device__ __forceinline__ uint32_t pack_pair(float x, float y, const __nv_bfloat16 *) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t pack_pair(float x, float y, const __half *) {
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t pack_pair(float, float, const float *) { return 0; }  // not reached
 
 struct Group {
   int32_t adapter;  // -1: none
@@ -295,14 +307,20 @@ struct LogitsPlan {
   uint32_t tiles_v;
   uint32_t stage;      // bytes
   uint32_t stages;
-  uint32_t acc;        // tensor memory columns of one accumulator
+  uint32_t acc;        // tensor memory columns of one half's accumulator
+  uint32_t buffers;    // sets of accumulators: with two, a tile's products run while the last one is stored
   // Bytes that a group of columns takes in a stage: for its adapter's rows, and
   // for its low-rank values per column; and how many columns fit.
   uint32_t group_rows, group_column, group_most;
 };
 
-struct alignas(8) LogitsShared {
+struct alignas(16) LogitsShared {
   uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
+  // By turns for every other tile: the token of a column (negative: none), and
+  // which columns' logits are NaN.
+  alignas(16) int32_t token[2][kMaxTileT];
+  uint32_t wrong[2][kMaxTileT / 32];
+  uint32_t more[2][kMaxTileT / 32];  // direct form: which columns' have a low-rank part
   uint32_t tmem, gave_up;
 };
 
@@ -313,12 +331,14 @@ LogitsPlan plan_logits(const ft_adapter_args &a, uint32_t columns, uint32_t part
   p.tile_t = ((columns + p.tiles_t - 1) / p.tiles_t + 15) / 16 * 16;
   p.acc = 32;
   while (p.acc < p.tile_t) p.acc *= 2;
-  // Two halves share the tokens' part of a stage, where two accumulators of
-  // each fit into the 512 columns and there are tiles enough for all SMs.
-  p.halves = p.acc <= 128 && a.vocab >= 148 * 4 * kTileV ? 2 : 1;
+  // Two halves share the tokens' part of a stage, where there are tiles enough
+  // for all SMs: an SM takes in 64 bytes a cycle, and one half by 256 columns
+  // needs 96 to keep the tensor cores busy, two need 64.
+  p.halves = a.vocab >= 148 * 4 * kTileV ? 2 : 1;
+  p.buffers = std::min<uint32_t>(2, 512 / (p.halves * p.acc));
   p.tiles_v = (a.vocab + p.halves * kTileV - 1) / (p.halves * kTileV);
   p.stage = (p.halves * kTileV + std::max(p.tile_t, 16 * parts)) * kTileD * 2;
-  p.stages = std::min<uint32_t>(kMaxStages, (225 * 1024) / p.stage);
+  p.stages = std::min<uint32_t>(kMaxStages, (220 * 1024) / p.stage);
   p.group_rows = p.halves * kTileV * width * 2;
   p.group_column = parts * width * 2;
   p.group_most = parts ? (p.stage - p.group_rows) / p.group_column / 16 * 16 : 0;
@@ -388,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_map(&map_w);
     prefetch_map(&map_h);
   }
-  if (warp == 9) tmem_alloc(&sh.tmem, 2 * p.halves * p.acc);
+  if (warp == kProductWarp) tmem_alloc(&sh.tmem, p.buffers * p.halves * p.acc);
   fence_before();
   __syncthreads();
   fence_after();
@@ -406,7 +426,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // then stays in uniform registers, from which these instructions take their
   // operands (a single lane alone needs 600 cycles a stage for moving them
   // there, more than the products of 128 columns take).
-  if (warp == 8) {
+  if (warp == kLoadWarp) {
     uint32_t at = 0, sent = 0;  // stage, and number of stages filled so far
     bool ok = true;
     auto open = [&] {  // the next stage, once it is free
@@ -459,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (uint32_t i = 0; i < kWaitTries && !mbar_try(&sh.full[s], fill & 1); ++i) {
         }
       }
-  } else if (warp == 9) {
+  } else if (warp == kProductWarp) {
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     uint32_t at = 0, phase = 0, n = 0;
     bool ok = true;
@@ -477,9 +497,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (uint32_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++n) {
       const Group mine = ahead;
       ahead = fetch(tile + gridDim.x);
-      const uint32_t b = n & 1, d = tmem + b * p.halves * p.acc, c0 = tile % tiles_t * p.tile_t;
+      const uint32_t b = n % p.buffers, d = tmem + b * p.halves * p.acc, c0 = tile % tiles_t * p.tile_t;
       const uint32_t shape = mma_shape(kBf16, kTileV, min(p.tile_t, (columns - c0 + 15) / 16 * 16));
-      if (n >= 2) ok = __all_sync(~0u, mbar_wait(&sh.acc_empty[b], (n / 2 - 1) & 1, gave_up));
+      if (n >= p.buffers) ok = __all_sync(~0u, mbar_wait(&sh.acc_empty[b], (n / p.buffers - 1) & 1, gave_up));
       if (!ok) break;
       fence_after();
       walk_tile(
@@ -521,28 +541,44 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok && elect_one()) mma_commit(&sh.acc_full[b]);
     }
   } else {
-    // Warps w and w + 4 read the same quarter of tensor memory (its lanes
-    // 32 (w % 4) on); they take one half of the vocabulary entries each, or
-    // alternate blocks of 16 columns.
+    // Warps with the same w % 4 read the same quarter of tensor memory (its
+    // lanes 32 (w % 4) on); they share the halves and the blocks of 16 columns.
     uint32_t n = 0;
     bool ok = true;
-    const uint32_t half = p.halves == 2 ? warp >> 2 : 0, row = half * kTileV + (warp & 3) * 32 + lane;
+    const uint32_t half = p.halves == 2 ? warp >> 3 : 0, row = half * kTileV + (warp & 3) * 32 + lane;
+    const uint32_t first = (p.halves == 2 ? warp >> 2 & 1 : warp >> 2) * 16, stride = p.halves == 2 ? 32 : 64;
+    const uint32_t odd = lane & 1;
     for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
-      const uint32_t b = n & 1, t0 = tile % tiles_t * p.tile_t;
+      const uint32_t b = n % p.buffers, t0 = tile % tiles_t * p.tile_t;
       const uint32_t v = tile / tiles_t * p.halves * kTileV + row;
       const bool live = v < a.vocab;
       const uint32_t count = min(p.tile_t, columns - t0);
-      if (ok) ok = mbar_wait(&sh.acc_full[b], (n / 2) & 1, gave_up);
+      if (threadIdx.x < kMaxTileT) {  // thread c looks up what column c is
+        const uint32_t c = threadIdx.x;
+        int32_t token = -1;
+        bool bad = false, more = false;
+        if (c < count) {
+          token = (int32_t)(t0 + c);
+          if (kSorted) {
+            token = o.col_token[t0 + c];
+            bad = token < -1;
+            if (bad) token = -2 - token;
+          } else if (delta) {
+            const int32_t id = a.adapter_ids[token / a.num_outpos];
+            more = (uint32_t)id < a.num_adapters;
+            bad = !more && id != -1;
+          }
+        }
+        sh.token[n & 1][c] = token;
+        const uint32_t bads = __ballot_sync(~0u, bad), mores = __ballot_sync(~0u, more);
+        if (lane == 0) sh.wrong[n & 1][warp] = bads, sh.more[n & 1][warp] = mores;
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(kEpilogue) : "memory");
+      const int32_t *tokens = sh.token[n & 1];
+      if (ok) ok = mbar_wait(&sh.acc_full[b], (n / p.buffers) & 1, gave_up);
       ok = __all_sync(~0u, ok);
       if (ok) fence_after();
-      for (uint32_t c0 = p.halves == 2 ? 0 : (warp >> 2) * 16; c0 < count; c0 += p.halves == 2 ? 16 : 32) {
-        // Lane e (and e + 16) looks up what column c0 + e is.
-        const uint32_t mine = t0 + c0 + (lane & 15);
-        int32_t token = -1, id = -1;
-        if (c0 + (lane & 15) < count) {
-          token = kSorted ? o.col_token[mine] : (int32_t)mine;
-          if (!kSorted && delta) id = a.adapter_ids[mine / a.num_outpos];
-        }
+      for (uint32_t c0 = first; c0 < count; c0 += stride) {
         uint32_t acc[16];
         if (ok) {
           tmem_load16(tmem + (b * p.halves + half) * p.acc + c0 + ((warp & 3) << 21), acc);
@@ -551,26 +587,46 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int e = 0; e < 16; ++e) acc[e] = 0x7FC00000;
         }
+        const uint32_t wrong = sh.wrong[n & 1][c0 / 32] >> (c0 % 32) & 0xFFFF;
         if (!kSorted && delta) {
-          const uint32_t any = __ballot_sync(~0u, (uint32_t)id < a.num_adapters);
-          const uint32_t wrong = __ballot_sync(~0u, (uint32_t)id >= a.num_adapters && id != -1);
-          float more[16];
+          const uint32_t any = sh.more[n & 1][c0 / 32] >> (c0 % 32) & 0xFFFF;
+          float add[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            more[e] = live && (any >> e & 1) ? __ldg(&delta[(uint64_t)(t0 + c0 + e) * a.vocab + v]) : 0.0f;
+            add[e] = live && (any >> e & 1) ? __ldg(&delta[(uint64_t)(t0 + c0 + e) * a.vocab + v]) : 0.0f;
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            acc[e] = wrong >> e & 1 ? 0x7FC00000 : __float_as_uint(__uint_as_float(acc[e]) + more[e]);
+          for (int e = 0; e < 16; ++e) acc[e] = __float_as_uint(__uint_as_float(acc[e]) + add[e]);
         }
+        if (wrong) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          int32_t to = __shfl_sync(~0u, token, e);
-          float y = __uint_as_float(acc[e]);
-          if (kSorted && to < -1) {
-            to = -2 - to;
-            y = __int_as_float(0x7FC00000);
+          for (int e = 0; e < 16; ++e)
+            if (wrong >> e & 1) acc[e] = 0x7FC00000;
+        }
+        int32_t to[16];
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const int4 q = *reinterpret_cast<const int4 *>(tokens + c0 + e);
+          to[e] = q.x, to[e + 1] = q.y, to[e + 2] = q.z, to[e + 3] = q.w;
+        }
+        uint8_t *out = static_cast<uint8_t *>(a.out) + (uint64_t)v * sizeof(O);
+        const uint32_t pitch = a.vocab * (uint32_t)sizeof(O);  // below 2^32, as is every token
+        if (sizeof(O) == 2 && a.vocab % 2 == 0) {
+          // Neighbouring lanes trade, so that each has two entries of one token
+          // and stores them together.
+          out -= odd * 2;
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) {
+            const uint32_t got = __shfl_xor_sync(~0u, odd ? acc[e] : acc[e + 1], 1);
+            const uint32_t two = pack_pair(__uint_as_float(odd ? got : acc[e]), __uint_as_float(odd ? acc[e + 1] : got),
+                                           static_cast<O *>(nullptr));
+            const int32_t t = odd ? to[e + 1] : to[e];
+            if (live && t >= 0) *reinterpret_cast<uint32_t *>(out + (uint64_t)(uint32_t)t * pitch) = two;
           }
-          if (live && to >= 0) from_f32(y, static_cast<O *>(a.out)[(uint64_t)to * a.vocab + v]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (live && to[e] >= 0)
+              from_f32(__uint_as_float(acc[e]), *reinterpret_cast<O *>(out + (uint64_t)(uint32_t)to[e] * pitch));
         }
       }
       if (ok) {
@@ -583,7 +639,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_before();
   __syncthreads();
   fence_after();
-  if (warp == 9) tmem_free(tmem, 2 * p.halves * p.acc);
+  if (warp == kProductWarp) tmem_free(tmem, p.buffers * p.halves * p.acc);
 }
 
 using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
@@ -639,7 +695,7 @@ void check_adapter(const ft_adapter_args &a) {
     throw InvalidArgument("adapter_logits: rank must be a multiple of 8 in [8, 256]");
   if (a.num_adapters > kMaxAdapters) throw InvalidArgument("adapter_logits: at most 65536 adapters");
   // Token and vocabulary coordinates of a tile are 32-bit.
-  if ((uint64_t)a.n * a.num_outpos > 0x3FFFFF || a.vocab > 0x7FFFFF00u || a.dim > 0xFFFFFF ||
+  if ((uint64_t)a.n * a.num_outpos > 0x3FFFFF || a.vocab > 0x3FFFFF00u || a.dim > 0xFFFFFF ||
       (uint64_t)(a.vocab / kTileV + 1) * ((uint64_t)a.n * a.num_outpos / 16 + 1) > 0x7FFFFFFF ||
       (uint64_t)(a.vocab / 256 + 1) * a.n > 0x7FFFFFFF)
     throw InvalidArgument("adapter_logits: too many tokens or too large a vocabulary");
