@@ -79,6 +79,9 @@ struct Sorted {
   uint32_t columns;      // upper bound, a multiple of 16
   uint32_t parts;
   uint32_t width;        // low-rank rows that a product's operands hold side by side: 16, 32 or 64
+  // One request: its tokens are in order as they are. There are no tables and
+  // no moved tokens; only u is written.
+  bool single;
 };
 
 // Sum over the items of the threads before this one, and over all.
@@ -189,7 +192,11 @@ __global__ void __launch_bounds__(256) shrink_kernel(ft_adapter_args a, float *u
   const T *h = static_cast<const T *>(a.hidden) + tok * a.dim;
   const uint32_t lane = threadIdx.x & 31;
   uint32_t col = 0;
-  if (kSorted) {
+  sm100::launch_next();
+  if (kSorted && o.single) {
+    col = l0;
+    if (!has) return;
+  } else if (kSorted) {
     col = o.req_col[req] + l0;
     uint4 *to = reinterpret_cast<uint4 *>(static_cast<T *>(o.hidden) + (uint64_t)col * a.dim);
     const uint4 *from = reinterpret_cast<const uint4 *>(h);
@@ -269,6 +276,7 @@ constexpr int kExpandThreads = 256, kExpandTokens = 8;
 // tokens of one request, so that an adapter's rows are read once a request.
 template <typename T>
 __global__ void __launch_bounds__(kExpandThreads) expand_kernel(ft_adapter_args a, const float *u, float *delta) {
+  sm100::launch_next();
   const uint32_t blocks = (a.vocab + kExpandThreads - 1) / kExpandThreads;
   const uint32_t req = blockIdx.x / blocks, v = blockIdx.x % blocks * kExpandThreads + threadIdx.x;
   const int32_t id = a.adapter_ids[req];
@@ -396,9 +404,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ LogitsShared sh;
   const uint32_t warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t bytes_w = p.halves * kTileV * kTileD * 2, bytes = p.stage;
-  const uint32_t columns = kSorted ? o.head[1] : p.columns;
-  const uint32_t tiles_t = (columns + p.tile_t - 1) / p.tile_t;
-  const uint32_t tiles = tiles_t * p.tiles_v, chunks = (a.dim + kTileD - 1) / kTileD;
   volatile uint32_t *gave_up = &sh.gave_up;
   if (threadIdx.x == 0) {
     sh.gave_up = 0;
@@ -413,11 +418,21 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   fence_after();
   const uint32_t tmem = sh.tmem;
+  // What the kernel before this one left: the tables here, u where the loads
+  // come to it, the direct form's sums in the epilogue.
+  const bool tables = kSorted && !o.single;
+  if (tables) wait_for_previous();
+  const uint32_t columns = tables ? o.head[1] : p.columns;
+  const uint32_t tiles_t = (columns + p.tile_t - 1) / p.tile_t;
+  const uint32_t tiles = tiles_t * p.tiles_v, chunks = (a.dim + kTileD - 1) / kTileD;
+  const int32_t only = kSorted && o.single ? a.adapter_ids[0] : -1;
 
   // A tile's groups, one a lane, are fetched while the tile before is under
   // way: a look into global memory takes microseconds when the memory is busy,
   // and neither loads nor products may pause for it.
   auto fetch = [&](uint32_t tile) {
+    if (kSorted && o.single)
+      return lane ? Group{-1, ~0u, ~0u, 0} : Group{(uint32_t)only < a.num_adapters ? only : -1, 0, columns, 0};
     return kSorted && lane < kTileGroups && tile < tiles ? o.tile_groups[tile % tiles_t * kTileGroups + lane]
                                                          : Group{-1, ~0u, ~0u, 0};
   };
@@ -456,7 +471,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             next();
             return true;
           },
-          open,
+          [&] {
+            if (o.single) wait_for_previous();
+            return open();
+          },
           [&](int32_t adapter, uint32_t w0, uint32_t w, uint32_t j, uint32_t offset) {
             uint8_t *st = buf + (size_t)at * bytes + offset;
             if (elect_one()) {
@@ -559,7 +577,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool bad = false, more = false;
         if (c < count) {
           token = (int32_t)(t0 + c);
-          if (kSorted) {
+          if (kSorted && o.single) {
+            bad = (uint32_t)only >= a.num_adapters && only != -1;
+            if (t0 + c >= a.num_outpos) token = -1;
+          } else if (kSorted) {
             token = o.col_token[t0 + c];
             bad = token < -1;
             if (bad) token = -2 - token;
@@ -575,6 +596,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       asm volatile("bar.sync 1, %0;" ::"n"(kEpilogue) : "memory");
       const int32_t *tokens = sh.token[n & 1];
+      if (!kSorted && delta && n == 0) wait_for_previous();
       if (ok) ok = mbar_wait(&sh.acc_full[b], (n / p.buffers) & 1, gave_up);
       ok = __all_sync(~0u, ok);
       if (ok) fence_after();
@@ -639,6 +661,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_before();
   __syncthreads();
   fence_after();
+  wait_for_previous();  // so that this kernel's end stands for that one's
   if (warp == kProductWarp) tmem_free(tmem, p.buffers * p.halves * p.acc);
 }
 
@@ -705,7 +728,7 @@ uint64_t align256(uint64_t x) { return (x + 255) & ~(uint64_t)255; }
 
 // Which form a call takes and where its workspace's parts lie.
 struct Layout {
-  bool sorted = false;
+  bool sorted = false, single = false;
   uint32_t tokens = 0, columns = 0, parts = 0, width = 0;
   uint64_t delta = 0, head = 0, groups = 0, tile_first = 0, tile_groups = 0, req_col = 0, col_token = 0, hidden = 0, u = 0, end = 0;
 };
@@ -718,8 +741,9 @@ Layout layout_of(const ft_adapter_args &a) {
   const uint64_t groups = std::min<uint64_t>(a.n, (uint64_t)a.num_adapters + 1);
   uint32_t step = 1;
   while (step < 16 && a.num_outpos % (2 * step) == 0) step *= 2;
-  const uint64_t most = ((uint64_t)l.tokens + groups * (16 - step) + 15) / 16 * 16;
-  l.sorted = a.n <= kMaxSortRequests && most <= 2 * (uint64_t)l.tokens;
+  l.single = a.n == 1;
+  const uint64_t most = ((uint64_t)l.tokens + (l.single ? 0 : groups * (16 - step)) + 15) / 16 * 16;
+  l.sorted = l.single || (a.n <= kMaxSortRequests && most <= 2 * (uint64_t)l.tokens);
   if (!l.sorted) {
     l.delta = align256((uint64_t)l.tokens * a.rank * 4);
     l.end = l.delta + align256((uint64_t)l.tokens * a.vocab * 4);
@@ -728,12 +752,17 @@ Layout layout_of(const ft_adapter_args &a) {
   l.columns = (uint32_t)most;
   l.width = a.rank <= 16 ? 16 : a.rank <= 32 ? 32 : 64;
   l.parts = a.dtype == FT_DTYPE_BF16 && a.out_dtype == FT_DTYPE_F32 ? 3 : 2;
-  uint64_t at = 256;
+  uint64_t at = l.single ? 0 : 256;
   auto place = [&](uint64_t bytes) {
     const uint64_t here = at;
     at += align256(bytes);
     return here;
   };
+  if (l.single) {
+    l.u = place((uint64_t)((a.rank + l.width - 1) / l.width) * most * l.parts * l.width * 2);
+    l.end = at;
+    return l;
+  }
   l.groups = place(sizeof(Group) * groups);
   l.tile_first = place(4 * (most / 16 + 1));
   l.tile_groups = place(sizeof(Group) * kTileGroups * (most / plan_logits(a, l.columns, l.parts, l.width).tile_t + 1));
@@ -777,16 +806,17 @@ void adapter_logits_device(const ft_adapter_args &a, void *ws, uint64_t ws_bytes
                reinterpret_cast<uint32_t *>(w + l.tile_first),
                reinterpret_cast<Group *>(w + l.tile_groups), reinterpret_cast<uint32_t *>(w + l.req_col),
                reinterpret_cast<int32_t *>(w + l.col_token), w + l.hidden,
-               w + l.u, l.columns, l.parts, l.width};
+               w + l.u, l.columns, l.parts, l.width, l.single};
   const bool bf16 = a.dtype == FT_DTYPE_BF16;
   const CUtensorMap map_w = make_map(a.weight, bf16, a.dim, a.vocab, 0, kTileD, p.halves * kTileV, "weight");
-  const CUtensorMap map_h = make_map(l.sorted ? o.hidden : a.hidden, bf16, a.dim, l.columns, 0, kTileD, p.tile_t, "hidden");
+  const CUtensorMap map_h = make_map(l.sorted && !l.single ? o.hidden : a.hidden, bf16, a.dim,
+                                     l.sorted && !l.single ? l.columns : l.tokens, 0, kTileD, p.tile_t, "hidden");
   CUtensorMap map_b = map_w;
   if (l.sorted) map_b = make_map(a.lora_b, bf16, a.rank, a.vocab, a.num_adapters, l.width, p.halves * kTileV, "lora_b");
   const size_t smem = logits_smem(p);
   const unsigned grid = std::min<unsigned>(p.tiles_t * p.tiles_v, (unsigned)sm_count());
   const unsigned shrink = a.n * ((a.num_outpos + kShrinkTokens - 1) / kShrinkTokens);
-  if (l.sorted) {
+  if (l.sorted && !l.single) {
     uint32_t slots = 2;
     while (slots < a.n) slots <<= 1;
     const size_t room = 16ull * slots;
@@ -797,8 +827,18 @@ void adapter_logits_device(const ft_adapter_args &a, void *ws, uint64_t ws_bytes
   }
   auto launch = [&](auto *kernel) {
     CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    kernel<<<grid, kThreads, smem, stream>>>(map_w, map_h, map_b, a, p, delta, o);
-    CUDA_TRY(cudaGetLastError());
+    // It may begin before the kernel that makes the low-rank values has ended.
+    cudaLaunchAttribute overlap;
+    overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    overlap.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = &overlap;
+    cfg.numAttrs = a.num_adapters ? 1 : 0;
+    CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, map_w, map_h, map_b, a, p, (const float *)delta, o));
   };
   auto run = [&](auto *t) {
     using T = std::remove_pointer_t<decltype(t)>;
