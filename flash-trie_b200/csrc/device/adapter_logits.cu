@@ -37,6 +37,7 @@ constexpr int kTileV = 128;   // vocabulary entries of one product's rows; a til
 constexpr int kTileD = 64;    // inner dimension of a stage: 128-byte rows
 constexpr int kMaxTileT = 256;
 constexpr int kMaxStages = 12;
+constexpr uint32_t kMaxParts = 3;
 constexpr int kEpilogue = 512;            // threads of warps 0-15; with half of them the stores take half as long again
 constexpr int kThreads = kEpilogue + 64;  // warp 16: loads, warp 17: products
 constexpr uint32_t kLoadWarp = kEpilogue / 32, kProductWarp = kLoadWarp + 1;
@@ -354,6 +355,11 @@ LogitsPlan plan_logits(const ft_adapter_args &a, uint32_t columns, uint32_t part
 }
 size_t logits_smem(const LogitsPlan &p) { return 1024 + (size_t)p.stages * p.stage; }
 
+// What a walk reads again and again, in registers.
+struct Walk {
+  uint32_t tile_t, stage, group_rows, group_column, group_most, width, slices, chunks;
+};
+
 // The stages of a tile in the order that loads and products both take them:
 // the shared projection's, then those of each group that has columns in it.
 // f(chunk) for the first, a stage each. The others share stages as far as they
@@ -362,24 +368,25 @@ size_t logits_smem(const LogitsPlan &p) { return 1024 + (size_t)p.stages * p.sta
 // callback that returns false ends the walk.
 // `mine`: the tile's groups, one a lane. The whole warp takes part.
 template <typename F, typename Open, typename G, typename Close>
-__device__ __forceinline__ bool walk_tile(const ft_adapter_args &a, const LogitsPlan &p, const Sorted &o, bool sorted,
-                                          const Group &mine, uint32_t c0, uint32_t chunks, F &&f, Open &&open, G &&g,
-                                          Close &&close) {
-  for (uint32_t c = 0; c < chunks; ++c)
+__device__ __forceinline__ bool walk_tile(const Walk &k, bool sorted, const Group &mine, uint32_t c0, F &&f, Open &&open,
+                                          G &&g, Close &&close) {
+  for (uint32_t c = 0; c < k.chunks; ++c)
     if (!f(c)) return false;
   if (!sorted) return true;
-  const uint32_t c1 = c0 + p.tile_t;
+  const uint32_t c1 = c0 + k.tile_t;
   uint32_t used = 0;
   for (uint32_t i = 0;; ++i) {
-    const uint32_t col0 = __shfl_sync(~0u, mine.col0, i), col1 = __shfl_sync(~0u, mine.col1, i);
-    const int32_t adapter = __shfl_sync(~0u, mine.adapter, i);
+    // A reduction rather than a shuffle: its result is uniform.
+    const bool from = (threadIdx.x & 31) == i;
+    const uint32_t col0 = __reduce_or_sync(~0u, from ? mine.col0 : 0), col1 = __reduce_or_sync(~0u, from ? mine.col1 : 0);
+    const int32_t adapter = (int32_t)__reduce_or_sync(~0u, from ? (uint32_t)mine.adapter : 0);
     if (col0 >= c1) break;  // the list ends with such a one
     if (adapter < 0) continue;
     const uint32_t end = min(col1, c1);
-    for (uint32_t w0 = max(col0, c0); w0 < end; w0 += p.group_most)
-      for (uint32_t j = 0; j * o.width < a.rank; ++j) {
-        const uint32_t w = min(p.group_most, end - w0), need = p.group_rows + w * p.group_column;
-        if (used && used + need > p.stage) {
+    for (uint32_t w0 = max(col0, c0); w0 < end; w0 += k.group_most)
+      for (uint32_t j = 0; j < k.slices; ++j) {
+        const uint32_t w = min(k.group_most, end - w0), need = k.group_rows + w * k.group_column;
+        if (used && used + need > k.stage) {
           close();
           used = 0;
         }
@@ -397,7 +404,8 @@ __device__ __forceinline__ bool walk_tile(const ft_adapter_args &a, const Logits
 template <typename T, typename O, bool kSorted>
 __global__ void __launch_bounds__(kThreads, 1)
     logits_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_h,
-                  const __grid_constant__ CUtensorMap map_b, ft_adapter_args a, LogitsPlan p, const float *delta, Sorted o) {
+                  const __grid_constant__ CUtensorMap map_b, const __grid_constant__ ft_adapter_args a,
+                  const __grid_constant__ LogitsPlan p, const float *delta, const __grid_constant__ Sorted o) {
   using namespace sm100;
   extern __shared__ uint8_t raw[];
   uint8_t *buf = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
@@ -424,7 +432,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (tables) wait_for_previous();
   const uint32_t columns = tables ? o.head[1] : p.columns;
   const uint32_t tiles_t = (columns + p.tile_t - 1) / p.tile_t;
-  const uint32_t tiles = tiles_t * p.tiles_v, chunks = (a.dim + kTileD - 1) / kTileD;
+  const uint32_t tiles = tiles_t * p.tiles_v;
+  const Walk walk{p.tile_t, p.stage, p.group_rows, p.group_column, p.group_most, o.width,
+                  kSorted ? (a.rank + o.width - 1) / o.width : 0, (a.dim + kTileD - 1) / kTileD};
   const int32_t only = kSorted && o.single ? a.adapter_ids[0] : -1;
 
   // A tile's groups, one a lane, are fetched while the tile before is under
@@ -437,13 +447,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                          : Group{-1, ~0u, ~0u, 0};
   };
 
-  // Both run as whole warps in step, one lane of which issues: what they count
-  // then stays in uniform registers, from which these instructions take their
-  // operands (a single lane alone needs 600 cycles a stage for moving them
-  // there, more than the products of 128 columns take).
+  const bool lead = elect_one();
   if (warp == kLoadWarp) {
     uint32_t at = 0, sent = 0;  // stage, and number of stages filled so far
     bool ok = true;
+    const uint8_t *low = o.u;
+    const uint32_t slice = o.columns;
     auto open = [&] {  // the next stage, once it is free
       if (sent >= p.stages) ok = mbar_wait(&sh.empty[at], (sent / p.stages - 1) & 1, gave_up);
       ok = __all_sync(~0u, ok);
@@ -459,15 +468,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       ahead = fetch(tile + gridDim.x);
       const int32_t v0 = (int32_t)(tile / tiles_t * p.halves * kTileV), t0 = (int32_t)(tile % tiles_t * p.tile_t);
       walk_tile(
-          a, p, o, kSorted, mine, (uint32_t)t0, chunks,
+          walk, kSorted, mine, (uint32_t)t0,
           [&](uint32_t c) {
             if (!open()) return false;
             uint8_t *st = buf + (size_t)at * bytes;
-            if (elect_one()) {
-              mbar_expect(&sh.full[at], bytes_w + p.tile_t * kTileD * 2);
-              tma_load_2d(st, &map_w, &sh.full[at], (int32_t)(c * kTileD), v0);
-              tma_load_2d(st + bytes_w, &map_h, &sh.full[at], (int32_t)(c * kTileD), t0);
-            }
+            mbar_expect(&sh.full[at], bytes_w + p.tile_t * kTileD * 2, lead);
+            tma_load_2d(st, &map_w, &sh.full[at], (int32_t)(c * kTileD), v0, lead);
+            tma_load_2d(st + bytes_w, &map_h, &sh.full[at], (int32_t)(c * kTileD), t0, lead);
             next();
             return true;
           },
@@ -477,15 +484,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           },
           [&](int32_t adapter, uint32_t w0, uint32_t w, uint32_t j, uint32_t offset) {
             uint8_t *st = buf + (size_t)at * bytes + offset;
-            if (elect_one()) {
-              mbar_expect_more(&sh.full[at], p.group_rows + w * p.group_column);
-              tma_load_3d(st, &map_b, &sh.full[at], (int32_t)(j * o.width), v0, adapter);
-              bulk_load(st + p.group_rows, o.u + ((uint64_t)j * o.columns + w0) * p.group_column, w * p.group_column,
-                        &sh.full[at]);
-            }
+            mbar_expect_more(&sh.full[at], walk.group_rows + w * walk.group_column, lead);
+            tma_load_3d(st, &map_b, &sh.full[at], (int32_t)(j * walk.width), v0, adapter, lead);
+            bulk_load(st + walk.group_rows, low + ((uint64_t)j * slice + w0) * walk.group_column, w * walk.group_column,
+                      &sh.full[at], lead);
           },
           [&] {
-            if (elect_one()) mbar_arrive(&sh.full[at]);
+            mbar_arrive(&sh.full[at], lead);
             next();
           });
     }
@@ -502,6 +507,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t at = 0, phase = 0, n = 0;
     bool ok = true;
     const uint64_t first_w = operand(buf), first_h = operand(buf + bytes_w);
+    const uint32_t parts = o.parts, rank = a.rank, halves = p.halves, acc = p.acc;
     auto open = [&] {
       ok = mbar_wait(&sh.full[at], phase, gave_up);
       ok = __all_sync(~0u, ok);
@@ -521,42 +527,48 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       fence_after();
       walk_tile(
-          a, p, o, kSorted, mine, c0, chunks,
+          walk, kSorted, mine, c0,
           [&](uint32_t c) {
             if (!open()) return false;
             const uint64_t w = first_w + (at * bytes >> 4), h = first_h + (at * bytes >> 4);
-            if (elect_one()) {
 #pragma unroll
-              for (int k = 0; k < kTileD / 16; ++k) mma_f16(d, w + 2 * k, h + 2 * k, shape, c > 0 || k > 0);
-              if (p.halves == 2) {
+            for (int k = 0; k < kTileD / 16; ++k) mma_f16(d, w + 2 * k, h + 2 * k, shape, c > 0 || k > 0, lead);
+            if (halves == 2) {
 #pragma unroll
-                for (int k = 0; k < kTileD / 16; ++k)
-                  mma_f16(d + p.acc, w + (kTileV * kTileD * 2 >> 4) + 2 * k, h + 2 * k, shape, c > 0 || k > 0);
-              }
-              mma_commit(&sh.empty[at]);
+              for (int k = 0; k < kTileD / 16; ++k)
+                mma_f16(d + acc, w + (kTileV * kTileD * 2 >> 4) + 2 * k, h + 2 * k, shape, c > 0 || k > 0, lead);
             }
+            mma_commit(&sh.empty[at], lead);
             done();
             return true;
           },
           open,
           [&](int32_t, uint32_t w0, uint32_t w, uint32_t j, uint32_t offset) {
-            const uint32_t row = o.width * 2;
+            // Loops over counts that are known here: with bounds looked up on the
+            // way every product took 160 cycles.
+            const uint32_t row = walk.width * 2;
             const uint8_t *st = buf + (size_t)at * bytes + offset;
-            const uint64_t bw = operand(st, row, 8 * row), uw = operand(st + p.group_rows, row, o.parts * 8 * row);
-            const uint32_t steps = (min(a.rank - j * o.width, o.width) + 15) / 16;
+            const uint64_t bw = operand(st, row, 8 * row), uw = operand(st + walk.group_rows, row, parts * 8 * row);
+            const uint32_t steps = (min(rank - j * walk.width, walk.width) + 15) / 16;
             const uint32_t narrow = mma_shape(kBf16, kTileV, w), to = d + (w0 - c0);
-            if (elect_one())
-              for (uint32_t half = 0; half < p.halves; ++half)
-                for (uint32_t x = 0; x < o.parts; ++x)
-                  for (uint32_t k = 0; k < steps; ++k)
-                    mma_f16(to + half * p.acc, bw + (half * kTileV * row >> 4) + 2 * k, uw + (x * 8 * row >> 4) + 2 * k,
-                            narrow, true);
+#pragma unroll
+            for (uint32_t k = 0; k < kTileD / 16; ++k)
+              if (k < steps) {
+#pragma unroll
+                for (uint32_t x = 0; x < kMaxParts; ++x)
+                  if (x < parts) {
+                    mma_f16(to, bw + 2 * k, uw + (x * 8 * row >> 4) + 2 * k, narrow, true, lead);
+                    if (halves == 2)
+                      mma_f16(to + acc, bw + (kTileV * row >> 4) + 2 * k, uw + (x * 8 * row >> 4) + 2 * k, narrow, true,
+                              lead);
+                  }
+              }
           },
           [&] {
-            if (elect_one()) mma_commit(&sh.empty[at]);
+            mma_commit(&sh.empty[at], lead);
             done();
           });
-      if (ok && elect_one()) mma_commit(&sh.acc_full[b]);
+      if (ok) mma_commit(&sh.acc_full[b], lead);
     }
   } else {
     // Warps with the same w % 4 read the same quarter of tensor memory (its
@@ -594,11 +606,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t bads = __ballot_sync(~0u, bad), mores = __ballot_sync(~0u, more);
         if (lane == 0) sh.wrong[n & 1][warp] = bads, sh.more[n & 1][warp] = mores;
       }
-      asm volatile("bar.sync 1, %0;" ::"n"(kEpilogue) : "memory");
+      // One warp looks for the products' end and the others wait at the block's
+      // barrier: sixteen warps that look would take the issue slots from the
+      // warps that load and multiply (160 instead of 70 cycles a product).
       const int32_t *tokens = sh.token[n & 1];
       if (!kSorted && delta && n == 0) wait_for_previous();
-      if (ok) ok = mbar_wait(&sh.acc_full[b], (n / p.buffers) & 1, gave_up);
-      ok = __all_sync(~0u, ok);
+      if (warp == 0 && ok) mbar_wait(&sh.acc_full[b], (n / p.buffers) & 1, gave_up);
+      asm volatile("bar.sync 1, %0;" ::"n"(kEpilogue) : "memory");
+      ok = __all_sync(~0u, ok && !*gave_up);
       if (ok) fence_after();
       for (uint32_t c0 = first; c0 < count; c0 += stride) {
         uint32_t acc[16];
