@@ -575,14 +575,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     // lanes 32 (w % 4) on); they share the halves and the blocks of 16 columns.
     uint32_t n = 0;
     bool ok = true;
-    const uint32_t half = p.halves == 2 ? warp >> 3 : 0, row = half * kTileV + (warp & 3) * 32 + lane;
-    const uint32_t first = (p.halves == 2 ? warp >> 2 & 1 : warp >> 2) * 16, stride = p.halves == 2 ? 32 : 64;
-    const uint32_t odd = lane & 1;
+    const uint32_t halves = p.halves, buffers = p.buffers, tile_t = p.tile_t, vocab = a.vocab;
+    const uint32_t half = halves == 2 ? warp >> 3 : 0, row = half * kTileV + (warp & 3) * 32 + lane;
+    const uint32_t first = (halves == 2 ? warp >> 2 & 1 : warp >> 2) * 16, stride = halves == 2 ? 32 : 64;
+    const uint32_t odd = lane & 1, pitch = vocab * (uint32_t)sizeof(O);  // below 2^32, as is every token
+    const bool pairs = sizeof(O) == 2 && vocab % 2 == 0;
+    const uint32_t mine = tmem + half * p.acc + ((warp & 3) << 21), set = halves * p.acc;
+    uint8_t *const logits = static_cast<uint8_t *>(a.out);
     for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
-      const uint32_t b = n % p.buffers, t0 = tile % tiles_t * p.tile_t;
-      const uint32_t v = tile / tiles_t * p.halves * kTileV + row;
-      const bool live = v < a.vocab;
-      const uint32_t count = min(p.tile_t, columns - t0);
+      const uint32_t b = n % buffers, t0 = tile % tiles_t * tile_t;
+      const uint32_t v = tile / tiles_t * halves * kTileV + row;
+      const bool live = v < vocab;
+      const uint32_t count = min(tile_t, columns - t0);
       if (threadIdx.x < kMaxTileT) {  // thread c looks up what column c is
         const uint32_t c = threadIdx.x;
         int32_t token = -1;
@@ -611,14 +615,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       // warps that load and multiply (160 instead of 70 cycles a product).
       const int32_t *tokens = sh.token[n & 1];
       if (!kSorted && delta && n == 0) wait_for_previous();
-      if (warp == 0 && ok) mbar_wait(&sh.acc_full[b], (n / p.buffers) & 1, gave_up);
+      if (warp == 0 && ok) mbar_wait(&sh.acc_full[b], (n / buffers) & 1, gave_up);
       asm volatile("bar.sync 1, %0;" ::"n"(kEpilogue) : "memory");
       ok = __all_sync(~0u, ok && !*gave_up);
       if (ok) fence_after();
       for (uint32_t c0 = first; c0 < count; c0 += stride) {
         uint32_t acc[16];
         if (ok) {
-          tmem_load16(tmem + (b * p.halves + half) * p.acc + c0 + ((warp & 3) << 21), acc);
+          tmem_load16(mine + b * set + c0, acc);
         } else {
           // A wait ran out: no result is better than a wrong one.
 #pragma unroll
@@ -630,7 +634,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           float add[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            add[e] = live && (any >> e & 1) ? __ldg(&delta[(uint64_t)(t0 + c0 + e) * a.vocab + v]) : 0.0f;
+            add[e] = live && (any >> e & 1) ? __ldg(&delta[(uint64_t)(t0 + c0 + e) * vocab + v]) : 0.0f;
 #pragma unroll
           for (int e = 0; e < 16; ++e) acc[e] = __float_as_uint(__uint_as_float(acc[e]) + add[e]);
         }
@@ -645,9 +649,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int4 q = *reinterpret_cast<const int4 *>(tokens + c0 + e);
           to[e] = q.x, to[e + 1] = q.y, to[e + 2] = q.z, to[e + 3] = q.w;
         }
-        uint8_t *out = static_cast<uint8_t *>(a.out) + (uint64_t)v * sizeof(O);
-        const uint32_t pitch = a.vocab * (uint32_t)sizeof(O);  // below 2^32, as is every token
-        if (sizeof(O) == 2 && a.vocab % 2 == 0) {
+        uint8_t *out = logits + (uint64_t)v * sizeof(O);
+        if (pairs) {
           // Neighbouring lanes trade, so that each has two entries of one token
           // and stores them together.
           out -= odd * 2;
