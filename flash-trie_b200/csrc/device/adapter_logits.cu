@@ -62,6 +62,23 @@ __device__ __forceinline__ uint32_t pack_pair(float x, float y, const __half *) 
 }
 __device__ __forceinline__ uint32_t pack_pair(float, float, const float *) { return 0; }  // not reached
 
+// Stores under a predicate: as branches, one after the other, they take twice as
+// long (690 and 340 cycles for 16 columns).
+__device__ __forceinline__ void store_if(bool yes, uint32_t *to, uint32_t x) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %0, 0;\n\t@q st.global.b32 [%1], %2;\n\t}" ::"r"((uint32_t)yes), "l"(to),
+               "r"(x));
+}
+__device__ __forceinline__ void store_if(bool yes, float *to, float x) {
+  store_if(yes, reinterpret_cast<uint32_t *>(to), __float_as_uint(x));
+}
+template <typename T>
+__device__ __forceinline__ void store_if(bool yes, T *to, float x) {
+  T h;
+  from_f32(x, h);
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %0, 0;\n\t@q st.global.b16 [%1], %2;\n\t}" ::"r"((uint32_t)yes), "l"(to),
+               "h"(*reinterpret_cast<const uint16_t *>(&h)));
+}
+
 struct Group {
   int32_t adapter;  // -1: none
   uint32_t col0, col1, pad;
@@ -325,9 +342,9 @@ struct LogitsPlan {
 
 struct alignas(16) LogitsShared {
   uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
-  // By turns for every other tile: the token of a column (negative: none), and
-  // which columns' logits are NaN.
-  alignas(16) int32_t token[2][kMaxTileT];
+  // By turns for every other tile: where a column's logits begin in the output
+  // (in bytes; negative: it has none), and which columns' logits are NaN.
+  int64_t begin[2][kMaxTileT];
   uint32_t wrong[2][kMaxTileT / 32];
   uint32_t more[2][kMaxTileT / 32];  // direct form: which columns' have a low-rank part
   uint32_t tmem, gave_up;
@@ -578,7 +595,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t halves = p.halves, buffers = p.buffers, tile_t = p.tile_t, vocab = a.vocab;
     const uint32_t half = halves == 2 ? warp >> 3 : 0, row = half * kTileV + (warp & 3) * 32 + lane;
     const uint32_t first = (halves == 2 ? warp >> 2 & 1 : warp >> 2) * 16, stride = halves == 2 ? 32 : 64;
-    const uint32_t odd = lane & 1, pitch = vocab * (uint32_t)sizeof(O);  // below 2^32, as is every token
+    const uint32_t odd = lane & 1;
+    const int64_t pitch = (int64_t)vocab * sizeof(O);
     const bool pairs = sizeof(O) == 2 && vocab % 2 == 0;
     const uint32_t mine = tmem + half * p.acc + ((warp & 3) << 21), set = halves * p.acc;
     uint8_t *const logits = static_cast<uint8_t *>(a.out);
@@ -606,14 +624,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             bad = !more && id != -1;
           }
         }
-        sh.token[n & 1][c] = token;
+        sh.begin[n & 1][c] = token < 0 ? -1 : (int64_t)token * pitch;
         const uint32_t bads = __ballot_sync(~0u, bad), mores = __ballot_sync(~0u, more);
         if (lane == 0) sh.wrong[n & 1][warp] = bads, sh.more[n & 1][warp] = mores;
       }
       // One warp looks for the products' end and the others wait at the block's
       // barrier: sixteen warps that look would take the issue slots from the
       // warps that load and multiply (160 instead of 70 cycles a product).
-      const int32_t *tokens = sh.token[n & 1];
+      const int64_t *begin = sh.begin[n & 1];
       if (!kSorted && delta && n == 0) wait_for_previous();
       if (warp == 0 && ok) mbar_wait(&sh.acc_full[b], (n / buffers) & 1, gave_up);
       asm volatile("bar.sync 1, %0;" ::"n"(kEpilogue) : "memory");
@@ -643,30 +661,30 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int e = 0; e < 16; ++e)
             if (wrong >> e & 1) acc[e] = 0x7FC00000;
         }
-        int32_t to[16];
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-          const int4 q = *reinterpret_cast<const int4 *>(tokens + c0 + e);
-          to[e] = q.x, to[e + 1] = q.y, to[e + 2] = q.z, to[e + 3] = q.w;
-        }
         uint8_t *out = logits + (uint64_t)v * sizeof(O);
         if (pairs) {
           // Neighbouring lanes trade, so that each has two entries of one token
           // and stores them together.
           out -= odd * 2;
+          int64_t at[8];
+          uint32_t two[8];
 #pragma unroll
-          for (int e = 0; e < 16; e += 2) {
-            const uint32_t got = __shfl_xor_sync(~0u, odd ? acc[e] : acc[e + 1], 1);
-            const uint32_t two = pack_pair(__uint_as_float(odd ? got : acc[e]), __uint_as_float(odd ? acc[e + 1] : got),
-                                           static_cast<O *>(nullptr));
-            const int32_t t = odd ? to[e + 1] : to[e];
-            if (live && t >= 0) *reinterpret_cast<uint32_t *>(out + (uint64_t)(uint32_t)t * pitch) = two;
+          for (int e = 0; e < 8; ++e) at[e] = begin[c0 + 2 * e + odd];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t got = __shfl_xor_sync(~0u, odd ? acc[2 * e] : acc[2 * e + 1], 1);
+            two[e] = pack_pair(__uint_as_float(odd ? got : acc[2 * e]), __uint_as_float(odd ? acc[2 * e + 1] : got),
+                               static_cast<O *>(nullptr));
           }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) store_if(live && at[e] >= 0, reinterpret_cast<uint32_t *>(out + at[e]), two[e]);
         } else {
+          int64_t at[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) at[e] = begin[c0 + e];
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            if (live && to[e] >= 0)
-              from_f32(__uint_as_float(acc[e]), *reinterpret_cast<O *>(out + (uint64_t)(uint32_t)to[e] * pitch));
+            store_if(live && at[e] >= 0, reinterpret_cast<O *>(out + at[e]), __uint_as_float(acc[e]));
         }
       }
       if (ok) {
