@@ -456,18 +456,42 @@ def _sequence_grad(logits, tokens, lengths, stats, grad, factor, upstream):
     return out
 
 
+def _scores(logits, tokens, lengths):
+    """(scores, what the gradient needs beside the inputs)"""
+    dev = logits.device
+    shape = _sequence_shape(logits, tokens)
+    logp = torch.empty(lengths.shape, dtype=torch.float32, device=dev)
+    stats = torch.empty((*shape[:2], 2), dtype=torch.float32, device=dev)
+    if logp.numel():
+        ws, ws_ptr, ws_bytes = _workspace(dev, "ft_sequence_logp_workspace", _SequenceArgs, *shape)
+        a = _SequenceArgs(*shape, logits.data_ptr(), tokens.data_ptr(), lengths.data_ptr(), stats.data_ptr(),
+                          logp.data_ptr(), None)
+        _check(_lib().ft_sequence_logp_device(ctypes.byref(a), ws_ptr, ws_bytes, _raw_stream(dev)))
+    return logp, stats
+
+
+def _preference(logits, tokens, lengths, ref_logp, chosen, rejected, beta, label_smoothing, mean):
+    """(loss, margin, what the gradient needs beside the inputs)"""
+    dev = logits.device
+    shape = _sequence_shape(logits, tokens)
+    stats = torch.empty((*shape[:2], 2), dtype=torch.float32, device=dev)
+    margin = torch.empty(chosen.shape, dtype=torch.float32, device=dev)
+    # Two tensors: a caller may change the loss in place before the backward pass.
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    factor = torch.empty((), dtype=torch.float32, device=dev)
+    grad = torch.empty(ref_logp.shape, dtype=torch.float32, device=dev)
+    ws, ws_ptr, ws_bytes = _workspace(dev, "ft_preference_loss_workspace", _SequenceArgs, *shape)
+    a = _SequenceArgs(*shape, logits.data_ptr(), tokens.data_ptr(), lengths.data_ptr(), stats.data_ptr(), None, None)
+    p = _PreferenceArgs(chosen.shape[1], int(mean), beta, label_smoothing, ref_logp.data_ptr(), chosen.data_ptr(),
+                        rejected.data_ptr(), margin.data_ptr(), loss.data_ptr(), grad.data_ptr(), factor.data_ptr())
+    _check(_lib().ft_preference_loss_device(ctypes.byref(a), ctypes.byref(p), ws_ptr, ws_bytes, _raw_stream(dev)))
+    return loss, margin, (stats, grad, factor)
+
+
 class _SequenceLogp(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, lengths):
-        dev = logits.device
-        shape = _sequence_shape(logits, tokens)
-        logp = torch.empty(lengths.shape, dtype=torch.float32, device=dev)
-        stats = torch.empty((*shape[:2], 2), dtype=torch.float32, device=dev)
-        if logp.numel():
-            ws, ws_ptr, ws_bytes = _workspace(dev, "ft_sequence_logp_workspace", _SequenceArgs, *shape)
-            a = _SequenceArgs(*shape, logits.data_ptr(), tokens.data_ptr(), lengths.data_ptr(), stats.data_ptr(),
-                              logp.data_ptr(), None)
-            _check(_lib().ft_sequence_logp_device(ctypes.byref(a), ws_ptr, ws_bytes, _raw_stream(dev)))
+        logp, stats = _scores(logits, tokens, lengths)
         ctx.save_for_backward(logits, tokens, lengths, stats)
         return logp
 
@@ -479,22 +503,9 @@ class _SequenceLogp(torch.autograd.Function):
 
 class _PreferenceLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, tokens, lengths, ref_logp, chosen, rejected, beta, label_smoothing, mean):
-        dev = logits.device
-        shape = _sequence_shape(logits, tokens)
-        stats = torch.empty((*shape[:2], 2), dtype=torch.float32, device=dev)
-        margin = torch.empty(chosen.shape, dtype=torch.float32, device=dev)
-        # Two tensors: a caller may change the loss in place before the backward pass.
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        factor = torch.empty((), dtype=torch.float32, device=dev)
-        grad = torch.empty(ref_logp.shape, dtype=torch.float32, device=dev)
-        ws, ws_ptr, ws_bytes = _workspace(dev, "ft_preference_loss_workspace", _SequenceArgs, *shape)
-        a = _SequenceArgs(*shape, logits.data_ptr(), tokens.data_ptr(), lengths.data_ptr(), stats.data_ptr(), None, None)
-        p = _PreferenceArgs(chosen.shape[1], int(mean), beta, label_smoothing, ref_logp.data_ptr(), chosen.data_ptr(),
-                            rejected.data_ptr(), margin.data_ptr(), loss.data_ptr(), grad.data_ptr(),
-                            factor.data_ptr())
-        _check(_lib().ft_preference_loss_device(ctypes.byref(a), ctypes.byref(p), ws_ptr, ws_bytes, _raw_stream(dev)))
-        ctx.save_for_backward(logits, tokens, lengths, stats, grad, factor)
+    def forward(ctx, logits, tokens, lengths, *rest):
+        loss, margin, more = _preference(logits, tokens, lengths, *rest)
+        ctx.save_for_backward(logits, tokens, lengths, *more)
         ctx.mark_non_differentiable(margin)
         ctx.set_materialize_grads(False)  # the margin's is not looked at
         return loss, margin
@@ -504,8 +515,7 @@ class _PreferenceLoss(torch.autograd.Function):
     def backward(ctx, g, _):
         if g is None:
             return (None,) * 9
-        *saved, grad, factor = ctx.saved_tensors
-        return (_sequence_grad(*saved, grad, factor, g),) + (None,) * 8
+        return (_sequence_grad(*ctx.saved_tensors, g),) + (None,) * 8
 
 
 def _want_candidates(logits, tokens, lengths):
@@ -538,7 +548,9 @@ def sequence_logp(logits, tokens, lengths, stream=None):
     backward pass runs on the forward call's stream."""
     dev = _want_candidates(logits, tokens, lengths)
     with _On(dev, stream):
-        return _SequenceLogp.apply(logits, tokens, lengths)
+        if logits.requires_grad and torch.is_grad_enabled():
+            return _SequenceLogp.apply(logits, tokens, lengths)
+        return _scores(logits, tokens, lengths)[0]
 
 
 def preference_loss(logits, tokens, lengths, ref_logp, chosen, rejected, beta=0.1, label_smoothing=0.0,
@@ -576,6 +588,8 @@ def preference_loss(logits, tokens, lengths, ref_logp, chosen, rejected, beta=0.
         raise ValueError("label_smoothing must be in [0, 1]")
     if reduction not in ("mean", "sum"):
         raise ValueError("reduction must be 'mean' or 'sum'")
+    args = (logits, tokens, lengths, ref_logp, chosen, rejected, beta, label_smoothing, reduction == "mean")
     with _On(dev, stream):
-        return _PreferenceLoss.apply(logits, tokens, lengths, ref_logp, chosen, rejected, beta, label_smoothing,
-                                     reduction == "mean")
+        if logits.requires_grad and torch.is_grad_enabled():
+            return _PreferenceLoss.apply(*args)
+        return _preference(*args)[:2]
