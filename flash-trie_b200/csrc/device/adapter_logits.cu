@@ -856,13 +856,12 @@ void adapter_logits_device(const ft_adapter_args &a, void *ws, uint64_t ws_bytes
     uint32_t slots = 2;
     while (slots < a.n) slots <<= 1;
     const size_t room = 16ull * slots;
-    if (room > 32 * 1024)
-      CUDA_TRY(cudaFuncSetAttribute(order_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)room));
+    allow_shared(order_kernel, 16 * (int)kMaxSortRequests);
     order_kernel<<<1, 1024, room, stream>>>(a.adapter_ids, a.n, a.num_outpos, a.num_adapters, slots, p.tile_t, o);
     CUDA_TRY(cudaGetLastError());
   }
   auto launch = [&](auto *kernel) {
-    CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    allow_shared(kernel, 221 * 1024);
     // It may begin before the kernel that makes the low-rank values has ended.
     cudaLaunchAttribute overlap;
     overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;

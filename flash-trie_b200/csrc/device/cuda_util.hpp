@@ -17,6 +17,15 @@ class CudaError : public std::runtime_error {
                   std::to_string(line) + ")");
 }
 
+// Lets a kernel have up to `most` bytes of dynamic shared memory. Every caller
+// of a kernel gives the same `most`: a smaller one would take effect for a call
+// that another thread is about to make.
+template <typename K>
+inline void allow_shared(K *kernel, int most) {
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  if (e != cudaSuccess) throw_cuda(e, "cudaFuncSetAttribute", __FILE__, __LINE__);
+}
+
 }  // namespace ftb
 
 #define CUDA_TRY(expr)                                                   \

@@ -516,8 +516,7 @@ void sequence_grad_device(const ft_sequence_args &a, const float *grad, const fl
   while (slots < 2 * a.candidates) slots <<= 1;
   const uint32_t threads = std::min<uint32_t>(1024, (a.candidates + 31) / 32 * 32);
   const size_t smem = 12ull * slots;
-  if (smem > 32 * 1024)
-    CUDA_TRY(cudaFuncSetAttribute(scatter_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  allow_shared(scatter_plan_kernel, 12 * 2 * kMaxCandidates);
   scatter_plan_kernel<<<(unsigned)p.rows, threads, smem, stream>>>(a.tokens, a.lengths, stats, grad, factor, upstream,
                                                                    a.vocab, a.num_outpos, a.candidates, slots, tok,
                                                                    tok_w, cnt, total);
@@ -564,8 +563,7 @@ void preference_loss_device(const ft_sequence_args &a, const ft_preference_args 
   uint32_t *ticket = reinterpret_cast<uint32_t *>(w + l.ticket);
   scores(a, w, lp, ticket, stream);
   const size_t smem = 8ull * a.candidates + 4 * ((a.candidates + 31) / 32);
-  if (smem > 32 * 1024)
-    CUDA_TRY(cudaFuncSetAttribute(pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  allow_shared(pair_kernel, 8 * kMaxCandidates + kMaxCandidates / 8);
   pair_kernel<<<a.n, kPairThreads, smem, stream>>>(p, a.n, a.candidates, lp, reinterpret_cast<double2 *>(w + l.part),
                                                    ticket);
   CUDA_TRY(cudaGetLastError());

@@ -550,7 +550,7 @@ void propose_device(const ft_propose_args &a, void *ws, uint64_t ws_bytes, cudaS
   const size_t smem = 8ull * l.p.cap + 4ull * l.p.hits;
   auto run = [&](auto *t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    CUDA_TRY(cudaFuncSetAttribute(propose_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    allow_shared(propose_kernel<T>, 225 * 1024 - (int)sizeof(Shared));
     propose_kernel<T><<<(unsigned)(a.rows * l.p.chunks), kThreads, smem, stream>>>(
         static_cast<const T *>(a.logits), a.vocab, a.topk, a.order, l.p, reinterpret_cast<SoftSum *>(w + l.part),
         reinterpret_cast<uint32_t *>(w + l.counts), reinterpret_cast<uint32_t *>(w + l.tickets),
