@@ -333,7 +333,8 @@ struct LogitsPlan {
   uint32_t tiles_v;
   uint32_t stage;      // bytes
   uint32_t stages;
-  uint32_t acc;        // tensor memory columns of one half's accumulator
+  uint32_t acc;        // tensor memory columns of an accumulator
+  uint32_t split;      // accumulators of a half: the inner dimension's chunks take turns
   uint32_t buffers;    // sets of accumulators: with two, a tile's products run while the last one is stored
   // Bytes that a group of columns takes in a stage: for its adapter's rows, and
   // for its low-rank values per column; and how many columns fit.
@@ -360,8 +361,13 @@ LogitsPlan plan_logits(const ft_adapter_args &a, uint32_t columns, uint32_t part
   // Two halves share the tokens' part of a stage, where there are tiles enough
   // for all SMs: an SM takes in 64 bytes a cycle, and one half by 256 columns
   // needs 96 to keep the tensor cores busy, two need 64.
-  p.halves = a.vocab >= 148 * 4 * kTileV ? 2 : 1;
-  p.buffers = std::min<uint32_t>(2, 512 / (p.halves * p.acc));
+  // The tensor cores cut each partial sum instead of rounding it, so that a sum
+  // of D products comes out D 5e-10 too small on average (1.6e-6 off, relative,
+  // at D = 2048): two sums of half the length are half as far off. 16-bit
+  // logits do not show it.
+  p.split = a.out_dtype == FT_DTYPE_F32 && a.dim > 1024 ? 2 : 1;
+  p.halves = a.vocab >= 148 * 4 * kTileV && (p.split == 1 || p.acc <= 64) ? 2 : 1;
+  p.buffers = std::min<uint32_t>(2, 512 / (p.halves * p.split * p.acc));
   p.tiles_v = (a.vocab + p.halves * kTileV - 1) / (p.halves * kTileV);
   p.stage = (p.halves * kTileV + std::max(p.tile_t, 16 * parts)) * kTileD * 2;
   p.stages = std::min<uint32_t>(kMaxStages, (220 * 1024) / p.stage);
@@ -438,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_map(&map_w);
     prefetch_map(&map_h);
   }
-  if (warp == kProductWarp) tmem_alloc(&sh.tmem, p.buffers * p.halves * p.acc);
+  if (warp == kProductWarp) tmem_alloc(&sh.tmem, p.buffers * p.halves * p.split * p.acc);
   fence_before();
   __syncthreads();
   fence_after();
@@ -524,7 +530,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t at = 0, phase = 0, n = 0;
     bool ok = true;
     const uint64_t first_w = operand(buf), first_h = operand(buf + bytes_w);
-    const uint32_t parts = o.parts, rank = a.rank, halves = p.halves, acc = p.acc;
+    const uint32_t parts = o.parts, rank = a.rank, halves = p.halves, acc = p.acc, split = p.split;
+    const uint32_t next_half = split * acc;
     auto open = [&] {
       ok = mbar_wait(&sh.full[at], phase, gave_up);
       ok = __all_sync(~0u, ok);
@@ -538,7 +545,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (uint32_t tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++n) {
       const Group mine = ahead;
       ahead = fetch(tile + gridDim.x);
-      const uint32_t b = n % p.buffers, d = tmem + b * p.halves * p.acc, c0 = tile % tiles_t * p.tile_t;
+      const uint32_t b = n % p.buffers, d = tmem + b * halves * next_half, c0 = tile % tiles_t * p.tile_t;
       const uint32_t shape = mma_shape(kBf16, kTileV, min(p.tile_t, (columns - c0 + 15) / 16 * 16));
       if (n >= p.buffers) ok = __all_sync(~0u, mbar_wait(&sh.acc_empty[b], (n / p.buffers - 1) & 1, gave_up));
       if (!ok) break;
@@ -548,12 +555,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           [&](uint32_t c) {
             if (!open()) return false;
             const uint64_t w = first_w + (at * bytes >> 4), h = first_h + (at * bytes >> 4);
+            const uint32_t turn = c & (split - 1), into = d + turn * acc;
+            const bool begun = c >= split;
 #pragma unroll
-            for (int k = 0; k < kTileD / 16; ++k) mma_f16(d, w + 2 * k, h + 2 * k, shape, c > 0 || k > 0, lead);
+            for (int k = 0; k < kTileD / 16; ++k) mma_f16(into, w + 2 * k, h + 2 * k, shape, begun || k > 0, lead);
             if (halves == 2) {
 #pragma unroll
               for (int k = 0; k < kTileD / 16; ++k)
-                mma_f16(d + acc, w + (kTileV * kTileD * 2 >> 4) + 2 * k, h + 2 * k, shape, c > 0 || k > 0, lead);
+                mma_f16(into + next_half, w + (kTileV * kTileD * 2 >> 4) + 2 * k, h + 2 * k, shape, begun || k > 0, lead);
             }
             mma_commit(&sh.empty[at], lead);
             done();
@@ -576,7 +585,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                   if (x < parts) {
                     mma_f16(to, bw + 2 * k, uw + (x * 8 * row >> 4) + 2 * k, narrow, true, lead);
                     if (halves == 2)
-                      mma_f16(to + acc, bw + (kTileV * row >> 4) + 2 * k, uw + (x * 8 * row >> 4) + 2 * k, narrow, true,
+                      mma_f16(to + next_half, bw + (kTileV * row >> 4) + 2 * k, uw + (x * 8 * row >> 4) + 2 * k, narrow, true,
                               lead);
                   }
               }
@@ -598,7 +607,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t odd = lane & 1;
     const int64_t pitch = (int64_t)vocab * sizeof(O);
     const bool pairs = sizeof(O) == 2 && vocab % 2 == 0;
-    const uint32_t mine = tmem + half * p.acc + ((warp & 3) << 21), set = halves * p.acc;
+    const uint32_t split = p.split, apart = p.acc, set = halves * split * apart;
+    const uint32_t mine = tmem + half * split * apart + ((warp & 3) << 21);
     uint8_t *const logits = static_cast<uint8_t *>(a.out);
     for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
       const uint32_t b = n % buffers, t0 = tile % tiles_t * tile_t;
@@ -641,6 +651,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t acc[16];
         if (ok) {
           tmem_load16(mine + b * set + c0, acc);
+          if (split == 2) {
+            uint32_t rest[16];
+            tmem_load16(mine + b * set + apart + c0, rest);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[e] = __float_as_uint(__uint_as_float(acc[e]) + __uint_as_float(rest[e]));
+          }
         } else {
           // A wait ran out: no result is better than a wrong one.
 #pragma unroll
@@ -698,7 +714,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   fence_after();
   wait_for_previous();  // so that this kernel's end stands for that one's
-  if (warp == kProductWarp) tmem_free(tmem, p.buffers * p.halves * p.acc);
+  if (warp == kProductWarp) tmem_free(tmem, p.buffers * p.halves * p.split * p.acc);
 }
 
 using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,

@@ -175,6 +175,39 @@ def test_propose_unaligned_rows_leave_neighbours_alone(fd):
         check_propose(fd, b[5:].view(1, 3, 1001), 40, "logp")
 
 
+def test_propose_all_equal(fd):
+    """Every logit passes any bound: the lowest ids win."""
+    x = torch.full((1, 2, 300001), 1.5, device="cuda")
+    for t in TYPES:
+        for k in (1, 1000, 8192):
+            check_propose(fd, x.to(t), k, "id")
+
+
+def test_propose_few_bounds_hold(fd):
+    """Rows whose best logits the sample sees too often or not at all."""
+    V = 262144
+    x = torch.randn((1, 4, V), generator=gen(3), device="cuda")
+    where = torch.arange(V, device="cuda")
+    x[0, 0, where % 128 < 16] += 9  # stretches of 16
+    x[0, 1, (where + 64) % 128 < 16] += 9
+    x[0, 2, :700] += 9
+    x[0, 3, where % 131 == 5] += 9
+    for t in TYPES:
+        check_propose(fd, x.to(t), 1200, "logp")
+
+
+def test_propose_beyond_2_31_entries(fd):
+    V, rows = 2200000, 1000
+    x = torch.empty((1, rows, V), dtype=torch.bfloat16, device="cuda").fill_(-4.0)
+    for l in (0, 976, 999):
+        x[0, l] = torch.randn(V, generator=gen(l), device="cuda").to(torch.bfloat16)
+    ids, lps = fd.propose(x, 100)
+    for l in (0, 976, 999):
+        want_ids, want = propose_oracle(x[:, l:l + 1], 100, "id")
+        assert torch.equal(ids[:, l:l + 1].cpu().long(), want_ids)
+    assert torch.equal(ids[0, 500].cpu().long(), torch.arange(100))
+
+
 def test_propose_no_rows(fd):
     ids, lps = fd.propose(torch.empty((0, 4, 10), device="cuda"), 3)
     assert ids.shape == lps.shape == (0, 4, 3)
@@ -279,6 +312,53 @@ def test_adapter_logits_same_bits_every_time(fd):
     for _ in range(3):
         assert torch.equal(first, fd.adapter_logits(h, w, ids, a, b, s, out_dtype=torch.float32))
     assert fd.adapter_logits(h[:0], w, ids[:0], a, b, s).shape == (0, 20, 5000)
+
+
+@pytest.mark.parametrize("t", HALVES)
+@pytest.mark.parametrize("n,L,V,D,r,G", [(1, 300, 80001, 72, 64, 1), (1, 1, 80000, 64, 8, 2), (20, 20, 76000, 136, 40, 6),
+                                         (3, 40, 90001, 1096, 16, 2), (2, 30, 76032, 1160, 72, 3),
+                                         (5, 60, 1001, 1032, 24, 2), (300, 1, 1000, 64, 8, 290), (9000, 1, 130, 16, 8, 3)])
+def test_adapter_logits_wide_and_long(fd, t, n, L, V, D, r, G):
+    """Vocabularies and batches that take two halves to a tile, several tiles
+    of tokens, long inner dimensions, slices of the low-rank dimension, groups
+    wider than a stage, and more requests than are sorted."""
+    h, w, ids, a, b, s = make_head(n, L, V, D, r, G, t, seed=n + V + D)
+    y, m = adapter_oracle(h, w, ids, a, b, s)
+    for out_t in (t, torch.float32):
+        check_adapter(fd.adapter_logits(h, w, ids, a, b, s, out_dtype=out_t), y, m, D, r, t)
+    y, m = adapter_oracle(h, w)
+    check_adapter(fd.adapter_logits(h, w, out_dtype=torch.float32), y, m, D, 0, t)
+
+
+@pytest.mark.parametrize("t", HALVES)
+@pytest.mark.parametrize("n,L,G", [(6, 20, 3), (6, 1, 6), (1, 5, 2)])
+def test_adapter_infinities_stay_with_their_requests(fd, t, n, L, G):
+    """An adapter whose B holds infinities and NaN reaches the requests that
+    use it, at those vocabulary entries, and nothing else."""
+    h, w, ids, a, b, s = make_head(n, L, 400, 64, 16, G, t, seed=12)
+    ids = (torch.arange(n, device="cuda") % G).to(torch.int32)
+    b[0, 7, 3] = math.inf
+    b[0, 200:210] = math.nan
+    y, m = adapter_oracle(h, w, ids, a, b, s)
+    out = fd.adapter_logits(h, w, ids, a, b, s)
+    wild = torch.zeros(400, dtype=torch.bool, device="cuda")
+    wild[7] = True
+    wild[200:210] = True
+    touched = (ids == 0)[:, None, None] & wild
+    assert not bool(torch.isfinite(out[touched.expand_as(out)]).any())
+    clean = ~touched.expand_as(out)
+    check_adapter(out[clean], y[clean], m[clean], 64, 16, t)
+
+
+def test_adapter_logits_beyond_2_31_entries(fd):
+    """Offsets of the last tokens pass 32 bits."""
+    V, D, n, L = 1100000, 64, 100, 20
+    h, w, ids, a, b, s = make_head(n, L, V, D, 8, 2, torch.bfloat16, seed=13)
+    out = fd.adapter_logits(h, w, ids, a, b, s)
+    assert out.numel() > 2 ** 31
+    for i in (0, 98, 99):
+        y, m = adapter_oracle(h[i:i + 1], w, ids[i:i + 1], a, b, s)
+        check_adapter(out[i:i + 1], y, m, D, 8, torch.bfloat16)
 
 
 # ------------------------------------------- sequence_logp, preference_loss
@@ -474,7 +554,7 @@ def test_preference_pairs_out_of_range(fd):
     c = torch.tensor([[0, -1, 1], [2, 3, -1]], dtype=torch.int32, device="cuda")
     r = torch.tensor([[1, 0, 4], [3, -5, -1]], dtype=torch.int32, device="cuda")
     loss, margin = fd.preference_loss(x, toks, lens, ref, c, r)
-    assert math.isnan(float(loss)) and math.isnan(float(margin[0, 2]))
+    assert math.isnan(float(loss.detach())) and math.isnan(float(margin[0, 2]))
     assert bool(torch.isfinite(margin.flatten()[[0, 1, 3, 4, 5]]).all()) and float(margin[0, 1]) == 0.0
     (dx,) = torch.autograd.grad(loss, x)
     assert bool(torch.isfinite(dx).all())
@@ -550,6 +630,29 @@ def test_gradient_is_the_same_every_time(fd):
         if first is None:
             first = got
         assert all(torch.equal(p, q) for p, q in zip(first, got))
+
+
+def test_sequence_logp_beyond_2_31_entries(fd):
+    V, L = 2200000, 1000
+    x = torch.randn((1, L, V), generator=gen(5), device="cuda", dtype=torch.bfloat16).requires_grad_()
+    toks, lens = make_candidates(1, L, V, 6, seed=6)
+    lens[:] = torch.tensor([L, L, 3, 0, 990, L], dtype=torch.int32)
+    lp = fd.sequence_logp(x, toks, lens)
+    w = torch.randn((1, 6), generator=gen(1), device="cuda")
+    (dx,) = torch.autograd.grad(lp, x, w)
+    for l0 in (0, 980):  # the first and the last positions
+        xd = x.detach()[:, l0:l0 + 20].double()
+        part = toks[:, :, l0:l0 + 20].contiguous()
+        _, live, at = sequence_oracle(xd, part, (lens - l0).clamp(0, 20))
+        check_gradient(dx[:, l0:l0 + 20], xd, live, at, w.double(), torch.bfloat16)
+    xs = x.detach()[0, :, :].float()
+    lse = torch.logsumexp(xs[990:], -1).double()
+    del xs
+    tail = x.detach()[0, 990:].gather(1, toks[0, 0, 990:, None].long())[:, 0].double() - lse
+    short = fd.sequence_logp(x.detach(), toks, torch.full_like(lens, 990))
+    # The two scores differ by the last ten positions; each was rounded once.
+    tol = 2 * U * float(lp[0, 0].detach().abs()) + 10 * (V / 32 + 200) * U
+    assert abs(float(lp[0, 0].detach()) - float(short[0, 0]) - float(tail.sum())) <= tol
 
 
 def test_sequence_logp_shapes_without_work(fd):
