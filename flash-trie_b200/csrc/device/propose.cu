@@ -259,18 +259,28 @@ __device__ float sample_bound(Shared &sh, const RowVecs<T> &r, uint32_t k) {
   constexpr int N = RowVecs<T>::N, kLoads = 4;
   const int64_t vecs = r.count();
   const int loads = (int)max((int64_t)1, min((int64_t)kLoads, vecs / (2 * kThreads))), parts = loads * kThreads / 8;
-  uint32_t key[kLoads][N];
+  const int64_t each = vecs / parts;
   uint4 q[kLoads];
   int64_t at[kLoads];
+#pragma unroll
+  for (int u = 0; u < kLoads; ++u) {
+    const int part = (u * kThreads + (int)threadIdx.x) / 8;
+    at[u] = u < loads ? part * each + each / 2 + threadIdx.x % 8 : vecs;  // vecs: nothing
+    if (r.whole(at[u])) q[u] = r.load_whole(at[u]);
+  }
   for (uint32_t b = threadIdx.x; b < kBins; b += kThreads) sh.hist[b] = 0;
   if (threadIdx.x == 0) sh.low32 = 0xFFFFFFFFu, sh.high32 = 0;
   __syncthreads();
-#pragma unroll
-  for (int u = 0; u < kLoads; ++u) {
-    const int64_t part = (u * kThreads + (int)threadIdx.x) / 8;
-    at[u] = u < loads ? vecs * (2 * part + 1) / (2 * parts) + threadIdx.x % 8 : vecs;  // vecs: nothing
-    if (r.whole(at[u])) q[u] = r.load_whole(at[u]);
-  }
+  // The k-th logit is expected at rank k (sample size) / V of the sample, give or
+  // take its square root; four of them and 4 more are left for safety (a row
+  // for which that is too few is read again).
+  const float rank = (float)k * (float)(loads * kThreads * N) / (float)r.len;
+  const uint32_t need = (uint32_t)(rank + 4.0f * sqrtf(rank)) + 4;
+  // The best `need` of the sample are hardly ever two in one vector while they
+  // are few: each vector's best then stands for it (an eighth of the work), and
+  // where two meet the bound is a little low.
+  const bool few = need <= kThreads / 8;
+  uint32_t key[kLoads][N];
   uint32_t low = 0xFFFFFFFFu, high = 0;
 #pragma unroll
   for (int u = 0; u < kLoads; ++u) {
@@ -279,8 +289,13 @@ __device__ float sample_bound(Shared &sh, const RowVecs<T> &r, uint32_t k) {
       unpack(q[u], v, (const T *)nullptr);
     else
       r.load_edge(at[u], v);
+    if (few) {
+#pragma unroll
+      for (int e = 1; e < N; ++e) v[0] = fmaxf(v[0], v[e]), v[e] = kNegInf;
+    }
 #pragma unroll
     for (int e = 0; e < N; ++e) {
+      if (few && e) break;
       key[u][e] = v[e] > kNegInf ? ordered(v[e]) : 0;
       if (key[u][e]) low = min(low, key[u][e]), high = max(high, key[u][e]);
     }
@@ -295,14 +310,12 @@ __device__ float sample_bound(Shared &sh, const RowVecs<T> &r, uint32_t k) {
 #pragma unroll
   for (int u = 0; u < kLoads; ++u)
 #pragma unroll
-    for (int e = 0; e < N; ++e)
+    for (int e = 0; e < N; ++e) {
+      if (few && e) break;
       if (key[u][e]) atomicAdd(&sh.hist[(key[u][e] - low) >> shift], 1u);
-  // The k-th logit is expected at rank k (sample size) / V of the sample, give or
-  // take its square root; four of them and 4 more are left for safety (a row
-  // for which that is too few is read again).
-  const float rank = (float)k * (float)(loads * kThreads * N) / (float)r.len;
+    }
   uint32_t bin, above;
-  find_bin(sh, (uint32_t)(rank + 4.0f * sqrtf(rank)) + 4, bin, above);
+  find_bin(sh, need, bin, above);
   if (bin == kBins) return kNegInf;
   return unordered(low + (bin << shift) - 1);  // the bin's least logit still passes
 }
@@ -418,16 +431,21 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
     }
     __syncthreads();
-    for (uint32_t c = 0; c < p.chunks; ++c) total += sh.hist[c];
+    uint32_t *before = sh.hist + 64;  // entries of the stretches before each
+    for (uint32_t c = 0; c < p.chunks; ++c) {
+      if (threadIdx.x == c) before[c] = total;
+      total += sh.hist[c];
+    }
+    __syncthreads();
     if (total <= p.cap) {
-      // A warp per stretch, each entry at its place.
-      for (uint32_t c = threadIdx.x >> 5; c < p.chunks; c += kThreads / 32) {
-        uint32_t at = 0;
-        for (uint32_t b = 0; b < c; ++b) at += sh.hist[b];
-        const Key *from = kept + (first + c) * p.emit;
-        const uint32_t have = sh.hist[c];
-#pragma unroll 8
-        for (uint32_t i = threadIdx.x & 31; i < have; i += 32) list[at + i] = __ldcg(&from[i]);
+      // Each entry to its place: most come from few stretches, so that the threads
+      // share all entries and look up where each one is.
+#pragma unroll 4
+      for (uint32_t i = threadIdx.x; i < total; i += kThreads) {
+        uint32_t c = 0;
+        for (uint32_t step = 32; step; step >>= 1)
+          if (c + step < p.chunks && before[c + step] <= i) c += step;
+        list[i] = __ldcg(&kept[(first + c) * p.emit + (i - before[c])]);
       }
       count = total;
     } else {

@@ -125,11 +125,11 @@ def _check(rc):
 
 
 def _want(t, name, dtype, ndim, device):
-    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError("%s must be a CUDA tensor" % name)
     if t.dtype != dtype or t.dim() != ndim or not t.is_contiguous():
         raise ValueError("%s must be a contiguous %s tensor with %d dimensions" % (name, dtype, ndim))
-    if device is not None and t.device != device:
+    if device is not None and t.get_device() != device.index:
         raise ValueError("%s is on %s, expected %s" % (name, t.device, device))
 
 
@@ -439,7 +439,7 @@ def _sequence_shape(logits, tokens):
 
 def _sequence_grad(logits, tokens, lengths, stats, grad, factor, upstream):
     """Gradient of the logits, on the current stream (autograd makes the
-    forward call's current)."""
+    forward call's current). stats, grad, factor, upstream: device pointers."""
     dev = logits.device
     with _On(dev, None):
         out = torch.empty_like(logits)
@@ -447,11 +447,8 @@ def _sequence_grad(logits, tokens, lengths, stats, grad, factor, upstream):
             return out.zero_()
         shape = _sequence_shape(logits, tokens)
         ws, ws_ptr, ws_bytes = _workspace(dev, "ft_sequence_logp_workspace", _SequenceArgs, *shape)
-        a = _SequenceArgs(*shape, logits.data_ptr(), tokens.data_ptr(), lengths.data_ptr(), stats.data_ptr(), None,
-                          out.data_ptr())
-        _check(_lib().ft_sequence_grad_device(ctypes.byref(a), grad.data_ptr(),
-                                              factor.data_ptr() if factor is not None else None,
-                                              upstream.data_ptr() if upstream is not None else None, ws_ptr, ws_bytes,
+        a = _SequenceArgs(*shape, logits.data_ptr(), tokens.data_ptr(), lengths.data_ptr(), stats, None, out.data_ptr())
+        _check(_lib().ft_sequence_grad_device(ctypes.byref(a), grad, factor, upstream, ws_ptr, ws_bytes,
                                               _raw_stream(dev)))
     return out
 
@@ -471,21 +468,23 @@ def _scores(logits, tokens, lengths):
 
 
 def _preference(logits, tokens, lengths, ref_logp, chosen, rejected, beta, label_smoothing, mean):
-    """(loss, margin, what the gradient needs beside the inputs)"""
+    """(loss, margin, what the gradient needs beside the inputs: the rows'
+    statistics, the candidates' gradients and their common factor in one
+    tensor)"""
     dev = logits.device
     shape = _sequence_shape(logits, tokens)
-    stats = torch.empty((*shape[:2], 2), dtype=torch.float32, device=dev)
+    n, L, C = shape[0], shape[1], shape[3]
     margin = torch.empty(chosen.shape, dtype=torch.float32, device=dev)
-    # Two tensors: a caller may change the loss in place before the backward pass.
     loss = torch.empty((), dtype=torch.float32, device=dev)
-    factor = torch.empty((), dtype=torch.float32, device=dev)
-    grad = torch.empty(ref_logp.shape, dtype=torch.float32, device=dev)
+    kept = torch.empty(2 * n * L + n * C + 1, dtype=torch.float32, device=dev)
     ws, ws_ptr, ws_bytes = _workspace(dev, "ft_preference_loss_workspace", _SequenceArgs, *shape)
-    a = _SequenceArgs(*shape, logits.data_ptr(), tokens.data_ptr(), lengths.data_ptr(), stats.data_ptr(), None, None)
+    at = kept.data_ptr()
+    a = _SequenceArgs(*shape, logits.data_ptr(), tokens.data_ptr(), lengths.data_ptr(), at, None, None)
     p = _PreferenceArgs(chosen.shape[1], int(mean), beta, label_smoothing, ref_logp.data_ptr(), chosen.data_ptr(),
-                        rejected.data_ptr(), margin.data_ptr(), loss.data_ptr(), grad.data_ptr(), factor.data_ptr())
+                        rejected.data_ptr(), margin.data_ptr(), loss.data_ptr(), at + 8 * n * L,
+                        at + 8 * n * L + 4 * n * C)
     _check(_lib().ft_preference_loss_device(ctypes.byref(a), ctypes.byref(p), ws_ptr, ws_bytes, _raw_stream(dev)))
-    return loss, margin, (stats, grad, factor)
+    return loss, margin, kept
 
 
 class _SequenceLogp(torch.autograd.Function):
@@ -498,14 +497,16 @@ class _SequenceLogp(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        return _sequence_grad(*ctx.saved_tensors, g.contiguous(), None, None), None, None
+        logits, tokens, lengths, stats = ctx.saved_tensors
+        g = g.contiguous()
+        return _sequence_grad(logits, tokens, lengths, stats.data_ptr(), g.data_ptr(), None, None), None, None
 
 
 class _PreferenceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, lengths, *rest):
-        loss, margin, more = _preference(logits, tokens, lengths, *rest)
-        ctx.save_for_backward(logits, tokens, lengths, *more)
+        loss, margin, kept = _preference(logits, tokens, lengths, *rest)
+        ctx.save_for_backward(logits, tokens, lengths, kept)
         ctx.mark_non_differentiable(margin)
         ctx.set_materialize_grads(False)  # the margin's is not looked at
         return loss, margin
@@ -515,7 +516,11 @@ class _PreferenceLoss(torch.autograd.Function):
     def backward(ctx, g, _):
         if g is None:
             return (None,) * 9
-        return (_sequence_grad(*ctx.saved_tensors, g),) + (None,) * 8
+        logits, tokens, lengths, kept = ctx.saved_tensors
+        n, L, C = logits.shape[0], logits.shape[1], tokens.shape[1]
+        at = kept.data_ptr()
+        return (_sequence_grad(logits, tokens, lengths, at, at + 8 * n * L, at + 8 * n * L + 4 * n * C,
+                               g.data_ptr()),) + (None,) * 8
 
 
 def _want_candidates(logits, tokens, lengths):
