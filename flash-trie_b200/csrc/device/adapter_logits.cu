@@ -288,40 +288,53 @@ __global__ void __launch_bounds__(256) shrink_kernel(ft_adapter_args a, float *u
   }
 }
 
-constexpr int kExpandThreads = 256, kExpandTokens = 8;
+constexpr int kExpandThreads = 256, kExpandRows = 4, kExpandTokens = 4;
 
-// The direct form's low-rank part: one vocabulary entry per thread for the
-// tokens of one request, so that an adapter's rows are read once a request.
+// The direct form's low-rank part: four vocabulary entries per thread, 256
+// apart, for the tokens of one request. What costs here is getting to the rows
+// of B, so that four are on their way at once; rows staged through shared
+// memory in whole lines came out three times slower.
 template <typename T>
 __global__ void __launch_bounds__(kExpandThreads) expand_kernel(ft_adapter_args a, const float *u, float *delta) {
   sm100::launch_next();
-  const uint32_t blocks = (a.vocab + kExpandThreads - 1) / kExpandThreads;
-  const uint32_t req = blockIdx.x / blocks, v = blockIdx.x % blocks * kExpandThreads + threadIdx.x;
+  const uint32_t blocks = (a.vocab + kExpandThreads * kExpandRows - 1) / (kExpandThreads * kExpandRows);
+  const uint32_t req = blockIdx.x / blocks, v0 = blockIdx.x % blocks * (kExpandThreads * kExpandRows) + threadIdx.x;
   const int32_t id = a.adapter_ids[req];
-  if ((uint32_t)id >= a.num_adapters || v >= a.vocab) return;
-  const T *b = static_cast<const T *>(a.lora_b) + ((uint64_t)id * a.vocab + v) * a.rank;
+  sm100::wait_for_previous();  // u
+  if ((uint32_t)id >= a.num_adapters) return;
+  const T *b = static_cast<const T *>(a.lora_b) + ((uint64_t)id * a.vocab + v0) * a.rank;
+  const uint64_t apart = (uint64_t)kExpandThreads * a.rank;
+  const uint32_t vocab = a.vocab, rank = a.rank;
   for (uint32_t l0 = 0; l0 < a.num_outpos; l0 += kExpandTokens) {
     const uint64_t t0 = (uint64_t)req * a.num_outpos + l0;
     const uint32_t count = min((uint32_t)kExpandTokens, a.num_outpos - l0);
-    float acc[kExpandTokens] = {};
-#pragma unroll 2
-    for (uint32_t r = 0; r < a.rank; r += 8) {
-      float w[8];
-      unpack8<T>(__ldg(reinterpret_cast<const uint4 *>(b + r)), w);
+    float acc[kExpandRows][kExpandTokens] = {};
+    for (uint32_t r = 0; r < rank; r += 8) {
+      uint4 q[kExpandRows];
 #pragma unroll
-      for (int q = 0; q < kExpandTokens; ++q) {
-        if (q >= (int)count) break;
-        const float4 *x = reinterpret_cast<const float4 *>(u + (t0 + q) * a.rank + r);
-        const float4 x0 = __ldg(x), x1 = __ldg(x + 1);
-        float s = acc[q];
-        s = fmaf(x0.x, w[0], s), s = fmaf(x0.y, w[1], s), s = fmaf(x0.z, w[2], s), s = fmaf(x0.w, w[3], s);
-        s = fmaf(x1.x, w[4], s), s = fmaf(x1.y, w[5], s), s = fmaf(x1.z, w[6], s), s = fmaf(x1.w, w[7], s);
-        acc[q] = s;
+      for (int i = 0; i < kExpandRows; ++i)
+        q[i] = v0 + i * kExpandThreads < vocab ? __ldg(reinterpret_cast<const uint4 *>(b + i * apart + r)) : uint4{};
+#pragma unroll
+      for (int x = 0; x < kExpandTokens; ++x) {
+        if (x >= (int)count) break;
+        const float4 *p = reinterpret_cast<const float4 *>(u + (t0 + x) * rank + r);
+        const float4 x0 = __ldcg(p), x1 = __ldcg(p + 1);
+#pragma unroll
+        for (int i = 0; i < kExpandRows; ++i) {
+          float w[8];
+          unpack8<T>(q[i], w);
+          float s = acc[i][x];
+          s = fmaf(x0.x, w[0], s), s = fmaf(x0.y, w[1], s), s = fmaf(x0.z, w[2], s), s = fmaf(x0.w, w[3], s);
+          s = fmaf(x1.x, w[4], s), s = fmaf(x1.y, w[5], s), s = fmaf(x1.z, w[6], s), s = fmaf(x1.w, w[7], s);
+          acc[i][x] = s;
+        }
       }
     }
 #pragma unroll
-    for (int q = 0; q < kExpandTokens; ++q)
-      if (q < (int)count) delta[(t0 + q) * a.vocab + v] = acc[q];
+    for (int i = 0; i < kExpandRows; ++i)
+#pragma unroll
+      for (int x = 0; x < kExpandTokens; ++x)
+        if (x < (int)count && v0 + i * kExpandThreads < vocab) delta[(t0 + x) * vocab + v0 + i * kExpandThreads] = acc[i][x];
   }
 }
 
@@ -717,6 +730,25 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kProductWarp) tmem_free(tmem, p.buffers * p.halves * p.split * p.acc);
 }
 
+// A launch that, with `early`, may begin before the kernel launched before it has
+// ended; it waits for that one itself. Only behind a kernel of the same call:
+// the call's inputs may come from whatever ran before that.
+template <typename... Params, typename... Args>
+void launch(bool early, unsigned grid, unsigned threads, size_t smem, cudaStream_t stream, void (*kernel)(Params...),
+            Args... args) {
+  cudaLaunchAttribute overlap;
+  overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  overlap.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &overlap;
+  cfg.numAttrs = early ? 1 : 0;
+  CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, args...));
+}
+
 using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
                               const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
                               CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -772,7 +804,7 @@ void check_adapter(const ft_adapter_args &a) {
   // Token and vocabulary coordinates of a tile are 32-bit.
   if ((uint64_t)a.n * a.num_outpos > 0x3FFFFF || a.vocab > 0x3FFFFF00u || a.dim > 0xFFFFFF ||
       (uint64_t)(a.vocab / kTileV + 1) * ((uint64_t)a.n * a.num_outpos / 16 + 1) > 0x7FFFFFFF ||
-      (uint64_t)(a.vocab / 256 + 1) * a.n > 0x7FFFFFFF)
+      (uint64_t)(a.vocab / kExpandThreads + 1) * a.n > 0x7FFFFFFF)
     throw InvalidArgument("adapter_logits: too many tokens or too large a vocabulary");
 }
 
@@ -795,7 +827,12 @@ Layout layout_of(const ft_adapter_args &a) {
   while (step < 16 && a.num_outpos % (2 * step) == 0) step *= 2;
   l.single = a.n == 1;
   const uint64_t most = ((uint64_t)l.tokens + (l.single ? 0 : groups * (16 - step)) + 15) / 16 * 16;
-  l.sorted = l.single || (a.n <= kMaxSortRequests && most <= 2 * (uint64_t)l.tokens);
+  // Padding costs products of the shared projection, the direct form products on
+  // the CUDA cores, r for each logit. 256 tokens by 100k x 1024, us sorted and
+  // direct: 64 groups of rank 64 (4.8 times the columns) 340 and 909, of rank 16
+  // 280 and 245; 64 of 4 tokens, rank 32 (4 times) 171 and 207; 100 of 2 tokens,
+  // rank 16 (8 times) 266 and 176.
+  l.sorted = l.single || (a.n <= kMaxSortRequests && 16 * most <= (uint64_t)l.tokens * (32 + a.rank));
   if (!l.sorted) {
     l.delta = align256((uint64_t)l.tokens * a.rank * 4);
     l.end = l.delta + align256((uint64_t)l.tokens * a.vocab * 4);
@@ -876,20 +913,9 @@ void adapter_logits_device(const ft_adapter_args &a, void *ws, uint64_t ws_bytes
     order_kernel<<<1, 1024, room, stream>>>(a.adapter_ids, a.n, a.num_outpos, a.num_adapters, slots, p.tile_t, o);
     CUDA_TRY(cudaGetLastError());
   }
-  auto launch = [&](auto *kernel) {
+  auto logits = [&](auto *kernel) {
     allow_shared(kernel, 221 * 1024);
-    // It may begin before the kernel that makes the low-rank values has ended.
-    cudaLaunchAttribute overlap;
-    overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    overlap.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cfg.attrs = &overlap;
-    cfg.numAttrs = a.num_adapters ? 1 : 0;
-    CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, map_w, map_h, map_b, a, p, (const float *)delta, o));
+    launch(a.num_adapters != 0, grid, kThreads, smem, stream, kernel, map_w, map_h, map_b, a, p, (const float *)delta, o);
   };
   auto run = [&](auto *t) {
     using T = std::remove_pointer_t<decltype(t)>;
@@ -899,14 +925,14 @@ void adapter_logits_device(const ft_adapter_args &a, void *ws, uint64_t ws_bytes
       shrink_kernel<T, false><<<shrink, 256, 0, stream>>>(a, u, o);
     CUDA_TRY(cudaGetLastError());
     if (u) {
-      const unsigned blocks = a.n * ((a.vocab + kExpandThreads - 1) / kExpandThreads);
-      expand_kernel<T><<<blocks, kExpandThreads, 0, stream>>>(a, u, delta);
-      CUDA_TRY(cudaGetLastError());
+      const uint32_t rows = kExpandThreads * kExpandRows;
+      launch(true, a.n * ((a.vocab + rows - 1) / rows), kExpandThreads, 0, stream, expand_kernel<T>, a, (const float *)u,
+             delta);
     }
     if (l.sorted)
-      a.out_dtype == FT_DTYPE_F32 ? launch(logits_kernel<T, float, true>) : launch(logits_kernel<T, T, true>);
+      a.out_dtype == FT_DTYPE_F32 ? logits(logits_kernel<T, float, true>) : logits(logits_kernel<T, T, true>);
     else
-      a.out_dtype == FT_DTYPE_F32 ? launch(logits_kernel<T, float, false>) : launch(logits_kernel<T, T, false>);
+      a.out_dtype == FT_DTYPE_F32 ? logits(logits_kernel<T, float, false>) : logits(logits_kernel<T, T, false>);
   };
   if (bf16)
     run((__nv_bfloat16 *)nullptr);
