@@ -52,7 +52,9 @@ RowPlan plan_rows(uint64_t rows, uint32_t vocab, int dtype) {
   return p;
 }
 
-// Partial (maximum, sum) of chunk blockIdx.y of row blockIdx.x.
+// Partial (maximum, sum) of chunk blockIdx.y of row blockIdx.x. Bound by the
+// logits' bytes: 35 us for 48 rows of 2.2M bf16 (211 MB, 6.0 TB/s) behind
+// kernels that left nothing to write back, 47 us behind a gradient of that size.
 template <typename T>
 __global__ void __launch_bounds__(kStatThreads)
     row_stats_kernel(const T *logits, uint32_t vocab, uint64_t vecs_chunk, SoftSum *part) {
@@ -68,7 +70,8 @@ __global__ void __launch_bounds__(kStatThreads)
 
 // Scores of 32 candidates of one request: eight lanes each, which take every
 // eighth position and add in 64 bits (a preference's margin is a small
-// difference of such sums).
+// difference of such sums). Latency of one look at the statistics and one at
+// each logit: 3 us for 10 candidates of 8 positions, 6.5 us for 1000 of 24.
 template <typename T>
 __global__ void __launch_bounds__(kScoreThreads)
     score_kernel(const T *logits, const uint32_t *tokens, const int32_t *lengths, uint32_t vocab, uint32_t L, uint32_t C,
@@ -309,8 +312,11 @@ __device__ __forceinline__ uint4 pack(const float (&v)[8], const __half *) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// The gradient of chunk blockIdx.y of row blockIdx.x: the softmax part first,
-// then, after the CTA's barrier, its tokens' entries over it.
+// The gradient of a chunk of row blockIdx.x: the softmax part first, then, after
+// the CTA's barrier, its tokens' entries over it. The chunks come in the
+// opposite order of the statistics', so that what those read last is still in
+// L2, and the gradient leaves it first: 73 -> 68 us for 48 rows of 2.2M bf16
+// (422 MB in and out, 6.2 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(kStatThreads)
     row_grad_kernel(const T *logits, T *grad, uint32_t vocab, uint32_t C, uint64_t vecs_chunk, const SoftSum *stats,
@@ -318,7 +324,7 @@ __global__ void __launch_bounds__(kStatThreads)
   constexpr int N = RowVecs<T>::N;
   const uint64_t row = blockIdx.x;
   const RowVecs<T> in(logits + row * vocab, vocab), out(grad + row * vocab, vocab);
-  const int64_t v0 = (int64_t)(blockIdx.y * vecs_chunk);
+  const int64_t v0 = (int64_t)((gridDim.y - 1 - blockIdx.y) * vecs_chunk);
   const int64_t v1 = min(v0 + (int64_t)vecs_chunk, out.count());
   T *g = grad + row * vocab;
   const SoftSum s = stats[row];
@@ -334,7 +340,7 @@ __global__ void __launch_bounds__(kStatThreads)
       const float2 y = mul2(k2, exp_below2(add2(make_float2(v[e], v[e + 1]), minus)));
       v[e] = y.x, v[e + 1] = y.y;
     }
-    *reinterpret_cast<uint4 *>(g + out.first(i)) = pack(v, (const T *)nullptr);
+    __stcs(reinterpret_cast<uint4 *>(g + out.first(i)), pack(v, (const T *)nullptr));
   };
   auto one_by_one = [&](int64_t i) {
 #pragma unroll
@@ -351,7 +357,7 @@ __global__ void __launch_bounds__(kStatThreads)
       if (zero) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          *reinterpret_cast<uint4 *>(g + out.first(i + u * kStatThreads)) = make_uint4(0, 0, 0, 0);
+          __stcs(reinterpret_cast<uint4 *>(g + out.first(i + u * kStatThreads)), make_uint4(0, 0, 0, 0));
       } else {
 #pragma unroll
         for (int u = 0; u < U; ++u) q[u] = in.load_whole(i + u * kStatThreads);
