@@ -301,7 +301,7 @@ def _workspace(device, *what):
 
 
 def _raw_stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch.cuda.current_stream(device.index).cuda_stream
 
 
 class _On:
@@ -371,7 +371,7 @@ def adapter_logits(hidden, weight, adapter_ids=None, lora_a=None, lora_b=None, s
     shape = (n, L, V, D, r, G, _DTYPE[dt], _DTYPE[out_dtype])
     with _On(dev, stream):
         ws, ws_ptr, ws_bytes = _workspace(dev, "ft_adapter_logits_workspace", _AdapterArgs, *shape)
-        out = torch.empty((n, L, V), dtype=out_dtype, device=dev)
+        out = torch.empty(n, L, V, dtype=out_dtype, device=dev)
         a = _AdapterArgs(*shape, hidden.data_ptr(), weight.data_ptr(), adapter_ids.data_ptr() if G else None,
                          lora_a.data_ptr() if G else None, lora_b.data_ptr() if G else None,
                          scale.data_ptr() if scale is not None else None, out.data_ptr())
@@ -405,8 +405,8 @@ def propose(logits, k, order="id", stream=None):
     _no_gradient("propose", logits=logits)
     shape = (n * L, V, k, _DTYPE[logits.dtype], int(order == "logp"))
     with _On(dev, stream):
-        ids = torch.empty((n, L, k), dtype=torch.int32, device=dev)
-        lps = torch.empty((n, L, k), dtype=torch.float32, device=dev)
+        ids = torch.empty(n, L, k, dtype=torch.int32, device=dev)
+        lps = torch.empty(n, L, k, dtype=torch.float32, device=dev)
         if n * L:
             ws, ws_ptr, ws_bytes = _workspace(dev, "ft_propose_workspace", _ProposeArgs, *shape)
             a = _ProposeArgs(*shape, logits.data_ptr(), ids.data_ptr(), lps.data_ptr())
@@ -457,8 +457,8 @@ def _scores(logits, tokens, lengths):
     """(scores, what the gradient needs beside the inputs)"""
     dev = logits.device
     shape = _sequence_shape(logits, tokens)
-    logp = torch.empty(lengths.shape, dtype=torch.float32, device=dev)
-    stats = torch.empty((*shape[:2], 2), dtype=torch.float32, device=dev)
+    logp = torch.empty(*lengths.shape, dtype=torch.float32, device=dev)
+    stats = torch.empty(*shape[:2], 2, dtype=torch.float32, device=dev)
     if logp.numel():
         ws, ws_ptr, ws_bytes = _workspace(dev, "ft_sequence_logp_workspace", _SequenceArgs, *shape)
         a = _SequenceArgs(*shape, logits.data_ptr(), tokens.data_ptr(), lengths.data_ptr(), stats.data_ptr(),
@@ -474,7 +474,7 @@ def _preference(logits, tokens, lengths, ref_logp, chosen, rejected, beta, label
     dev = logits.device
     shape = _sequence_shape(logits, tokens)
     n, L, C = shape[0], shape[1], shape[3]
-    margin = torch.empty(chosen.shape, dtype=torch.float32, device=dev)
+    margin = torch.empty(*chosen.shape, dtype=torch.float32, device=dev)
     loss = torch.empty((), dtype=torch.float32, device=dev)
     kept = torch.empty(2 * n * L + n * C + 1, dtype=torch.float32, device=dev)
     ws, ws_ptr, ws_bytes = _workspace(dev, "ft_preference_loss_workspace", _SequenceArgs, *shape)
