@@ -535,8 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!ok)
       for (uint32_t s = 0; s < p.stages && s < sent; ++s) {
         const uint32_t fill = (sent - 1 - s) / p.stages;
-        for (uint32_t i = 0; i < kWaitTries && !mbar_try(&sh.full[s], fill & 1); ++i) {
-        }
+        mbar_settle(&sh.full[s], fill & 1);
       }
   } else if (warp == kProductWarp) {
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
@@ -878,10 +877,11 @@ void adapter_logits_device(const ft_adapter_args &a, void *ws, uint64_t ws_bytes
     if (!p) fail(ErrorKind::kNull, "MARISA_NULL_ERROR: adapter_logits: hidden, weight or out is NULL");
   if (a.num_adapters && (!a.adapter_ids || !a.lora_a || !a.lora_b))
     fail(ErrorKind::kNull, "MARISA_NULL_ERROR: adapter_logits: adapter_ids, lora_a or lora_b is NULL");
-  const void *sixteen[] = {a.hidden, a.weight, a.num_adapters ? a.lora_a : nullptr, a.num_adapters ? a.lora_b : nullptr};
+  const void *sixteen[] = {a.hidden, a.weight, a.out, a.num_adapters ? a.lora_a : nullptr,
+                           a.num_adapters ? a.lora_b : nullptr};
   for (const void *p : sixteen)
     if (reinterpret_cast<uintptr_t>(p) & 15)
-      throw InvalidArgument("adapter_logits: hidden, weight, lora_a and lora_b must start on 16-byte boundaries");
+      throw InvalidArgument("adapter_logits: hidden, weight, lora_a, lora_b and out must start on 16-byte boundaries");
   const Layout l = layout_of(a);
   if (ws_bytes < l.end || (l.end && (!ws || (reinterpret_cast<uintptr_t>(ws) & 255))))
     throw InvalidArgument("adapter_logits: needs a 256-byte aligned workspace of " + std::to_string(l.end) + " bytes");

@@ -62,17 +62,32 @@ __device__ __forceinline__ bool mbar_try(uint64_t *bar, uint32_t parity) {
   return ok != 0;
 }
 
-// Waits for the phase, at most kWaitTries times the hardware's own time limit
-// (each try suspends the thread for up to some microseconds).  A wait that
-// runs out sets `gave_up`, which ends every other wait of the block early.
-constexpr uint32_t kWaitTries = 1u << 22;
+__device__ __forceinline__ uint64_t nanoseconds() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+  return t;
+}
+
+// Waits for the phase, two seconds at most (no tile takes a thousandth of
+// that). A wait that runs out sets `gave_up`, which ends every other wait of
+// the block.
+constexpr uint64_t kWaitLimit = 2000000000;
 __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, volatile uint32_t *gave_up) {
-  for (uint32_t i = 0; i < kWaitTries; ++i) {
+  for (int i = 0; i < 16; ++i)
     if (mbar_try(bar, parity)) return true;
-    if ((i & 1023) == 1023 && *gave_up) return false;
-  }
+  const uint64_t begin = nanoseconds();
+  do {
+    if (mbar_try(bar, parity)) return true;
+    if (*gave_up) return false;
+  } while (nanoseconds() - begin < kWaitLimit);
   *gave_up = 1;
   return false;
+}
+// The same for copies in flight when the block has given up already.
+__device__ __forceinline__ void mbar_settle(uint64_t *bar, uint32_t parity) {
+  const uint64_t begin = nanoseconds();
+  while (!mbar_try(bar, parity) && nanoseconds() - begin < kWaitLimit) {
+  }
 }
 
 // A kernel launched to overlap the one before it: everything that reads what

@@ -239,9 +239,10 @@ int ft_tbs_batch_device_noalloc(ft_trie *trie, const ft_device_batch *batch,
  *                + scale[a] sum_r (sum_d hidden[i][l][d] lora_a[a][r][d]) lora_b[a][v][r]
  * with a = adapter_ids[i].  a = -1: the shared projection alone; any other id
  * outside [0, num_adapters) makes the request's logits NaN.  hidden, weight,
- * lora_a and lora_b are dtype (bf16 or f16) and start on 16-byte boundaries;
- * dim and rank are multiples of 8, rank at most 256; out is out_dtype (the
- * same type, or f32).  num_adapters = 0: adapter_ids, lora_a, lora_b and
+ * lora_a and lora_b are dtype (bf16 or f16), out is out_dtype (the same type,
+ * or f32); all five start on 16-byte boundaries.  dim and rank are multiples
+ * of 8, rank at most 256.  With f16 operands scale * (hidden lora_a) must stay
+ * within f16's range (65504).  num_adapters = 0: adapter_ids, lora_a, lora_b and
  * scale are not read.  scale may be NULL (1 for every adapter).  At most
  * 65536 adapters.
  */

@@ -560,7 +560,7 @@ def test_preference_pairs_out_of_range(fd):
     assert bool(torch.isfinite(dx).all())
     none = torch.full_like(c, -1)
     loss, margin = fd.preference_loss(x, toks, lens, ref, none, none)
-    assert float(loss) == 0.0 and not bool(margin.any())
+    assert float(loss.detach()) == 0.0 and not bool(margin.any())
     (dx,) = torch.autograd.grad(loss, x)
     assert not bool(dx.any())
 
@@ -752,6 +752,61 @@ def test_captured_and_replayed_on_new_inputs(fd):
     for _, out, _ in graphs:
         assert all(torch.equal(p, q) for p, q in zip(want, out))
     del alive
+
+
+def test_two_threads_at_once(fd):
+    """Calls from two threads on streams of their own give what one thread
+    gets, whatever sizes the other one asks for."""
+    import threading
+    sets = [_inputs(71), _inputs(72, n=5, L=3, V=1201, D=128, r=8, G=2, C=300, P=40)]
+    want = [_calls(fd, *a)() for a in sets]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(which):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            run = _calls(fd, *sets[which])
+            for _ in range(20):
+                got = run()
+                stream.synchronize()
+                if not all(torch.equal(p, q) for p, q in zip(want[which], got)):
+                    wrong.append(which)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+def test_a_weight_that_is_no_number_stays_in_its_rows(fd):
+    """An upstream gradient of NaN makes NaN of the positions that its
+    candidate reaches, and of nothing else."""
+    x = make_logits(2, 6, 333, torch.float32, seed=3, masked=False).requires_grad_()
+    toks, lens = make_candidates(2, 6, 333, 9, seed=3)
+    lens[0, 4], lens[1, 4] = 3, 0
+    lp = fd.sequence_logp(x, toks, lens)
+    w = torch.randn((2, 9), generator=gen(3), device="cuda")
+    (clean,) = torch.autograd.grad(lp, x, w, retain_graph=True)
+    w[0, 4] = math.nan
+    (dx,) = torch.autograd.grad(lp, x, w)
+    assert bool(torch.isnan(dx[0, :3]).all())
+    assert torch.equal(dx[0, 3:], clean[0, 3:]) and torch.equal(dx[1], clean[1])
+
+
+def test_hidden_search_of_no_requests(fd, tmp_path):
+    import flashtrie
+    t = flashtrie.Trie()
+    t.build(token_rows=[[1, 2], [3]])
+    t.init_tbs_gpu(1, max_num_topk=8, max_num_outpos=4, max_num_out_beams=4)
+    h, w, ids, a, b, s = make_head(1, 4, 50, 64, 8, 2, torch.bfloat16, seed=1)
+    beams = torch.full((0, 4), 4, dtype=torch.int32, device="cuda")
+    out = fd.bs_tbs_hidden(t, beams, h[:0], w, 8, -10.0, -40.0, 1.0, False, ids[:0], a, b, s)
+    assert out[0].shape == (0,)
+    with pytest.raises(ValueError):
+        fd.bs_tbs_hidden(t, beams, h, w, 8, -10.0, -40.0, 1.0, False)
 
 
 def test_python_refusals(fd):

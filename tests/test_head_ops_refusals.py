@@ -67,7 +67,7 @@ def test_adapter_null_refused(fd, bad):
     assert fd._lib().ft_adapter_logits_device(ctypes.byref(a), P, 1 << 40, None) == NULL
 
 
-@pytest.mark.parametrize("bad", [dict(hidden=4098), dict(weight=4104), dict(lora_a=4098), dict(lora_b=4104)])
+@pytest.mark.parametrize("bad", [dict(hidden=4098), dict(weight=4104), dict(lora_a=4098), dict(lora_b=4104), dict(out=4098)])
 def test_adapter_unaligned_refused(fd, bad):
     a = adapter(fd, **{k: ctypes.c_void_p(v) for k, v in bad.items()})
     assert fd._lib().ft_adapter_logits_device(ctypes.byref(a), P, 1 << 40, None) == INVALID
