@@ -10,6 +10,7 @@
 // ones: a row's gradient is -W_l p[v], put right at the at most C distinct
 // tokens.  Both passes are bound by the bytes of the logits.
 #include <algorithm>
+#include <cmath>
 #include <string>
 
 #include "../engine.hpp"
@@ -546,6 +547,7 @@ void preference_loss_device(const ft_sequence_args &a, const ft_preference_args 
   check_sequence(a, "preference_loss");
   if (!(p.label_smoothing >= 0.0f && p.label_smoothing <= 1.0f))
     throw InvalidArgument("preference_loss: label_smoothing must be in [0, 1]");
+  if (!std::isfinite(p.beta)) throw InvalidArgument("preference_loss: beta must be finite");
   if (p.pairs >= 1u << 30) throw InvalidArgument("preference_loss: too many pairs per request");
   need_ptr(p.loss, "loss");
   need_ptr(p.factor, "factor");

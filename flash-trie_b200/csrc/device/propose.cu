@@ -317,7 +317,10 @@ __device__ float sample_bound(Shared &sh, const RowVecs<T> &r, uint32_t k) {
   uint32_t bin, above;
   find_bin(sh, need, bin, above);
   if (bin == kBins) return kNegInf;
-  return unordered(low + (bin << shift) - 1);  // the bin's least logit still passes
+  // The bin's least logit still passes. Below 0 comes the largest negative
+  // number, not -0, which 0 would not pass.
+  const uint32_t least = low + (bin << shift) - 1;
+  return unordered(least - (least == 0x7FFFFFFFu));
 }
 
 template <typename T>
@@ -454,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         const uint32_t have = __ldcg(&counts[first + c]);
         __syncthreads();
         count = sh.count;
-        if (count + have > p.cap) least = keep_largest(sh, list, count, k, 256);
+        if (count + have > p.cap) least = keep_largest(sh, list, count, k, 0);  // k + emit fit, no more
         __syncthreads();
         for (uint32_t i = threadIdx.x; i < have; i += kThreads) {
           const Key x = __ldcg(&kept[(first + c) * p.emit + i]);

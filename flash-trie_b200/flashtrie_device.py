@@ -309,6 +309,8 @@ class _On:
 
     def __init__(self, device, stream):
         self.inner = []
+        if stream is not None and stream.device_index != device.index:
+            raise ValueError("stream must be of the tensors' device, cuda:%d" % device.index)
         if torch.cuda.current_device() != device.index:
             self.inner.append(torch.cuda.device(device))
         if stream is not None:
@@ -335,6 +337,8 @@ def adapter_logits(hidden, weight, adapter_ids=None, lora_a=None, lora_b=None, s
     float32 [G] (default 1).  D and r are multiples of 8, r <= 256.  An id of
     -1 takes the shared projection alone; any other id outside [0, G) makes
     that request's logits NaN.  Without adapter_ids there are no adapters.
+    Infinities and NaN in an adapter reach its own requests only; where lora_b
+    or the product with lora_a is infinite the logit is NaN or infinite.
     Products are summed in 32 bits and rounded once.  Returns [n, L, V] of
     out_dtype (hidden's type, the default, or float32).  For serving: it has
     no gradient."""

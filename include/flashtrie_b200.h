@@ -242,7 +242,9 @@ int ft_tbs_batch_device_noalloc(ft_trie *trie, const ft_device_batch *batch,
  * lora_a and lora_b are dtype (bf16 or f16), out is out_dtype (the same type,
  * or f32); all five start on 16-byte boundaries.  dim and rank are multiples
  * of 8, rank at most 256.  With f16 operands scale * (hidden lora_a) must stay
- * within f16's range (65504).  num_adapters = 0: adapter_ids, lora_a, lora_b and
+ * within f16's range (65504), and is kept to 2^-25 absolute or better.  An
+ * infinite one, or an infinity in lora_b, makes the logits that it enters NaN
+ * or infinite.  out overlaps none of the inputs.  num_adapters = 0: adapter_ids, lora_a, lora_b and
  * scale are not read.  scale may be NULL (1 for every adapter).  At most
  * 65536 adapters.
  */
@@ -321,7 +323,8 @@ int ft_sequence_logp_workspace(const ft_sequence_args *args, uint64_t *bytes);
 int ft_sequence_logp_device(const ft_sequence_args *args, void *workspace, uint64_t workspace_bytes, void *stream);
 /* grad_logits = the gradient of sum_ij w[i][j] logp[i][j], with w = grad
  * ([n][candidates]), times *factor and *upstream (device scalars, each may be
- * NULL).  Reads stats as the forward call left it. */
+ * NULL).  Reads stats as the forward call left it; grad_logits may not overlap
+ * logits. */
 int ft_sequence_grad_device(const ft_sequence_args *args, const float *grad, const float *factor,
                             const float *upstream, void *workspace, uint64_t workspace_bytes, void *stream);
 
@@ -329,7 +332,7 @@ int ft_sequence_grad_device(const ft_sequence_args *args, const float *grad, con
  * Preference loss on pairs of candidates of the same request:
  *   margin = beta ((logp[c] - ref_logp[c]) - (logp[r] - ref_logp[r]))
  *   loss   = sum over pairs of (1 - s) softplus(-margin) + s softplus(margin),
- * s = label_smoothing; with `mean`, divided by the number of pairs (at least
+ * s = label_smoothing, in [0, 1]; beta is finite; with `mean`, divided by the number of pairs (at least
  * 1).  A pair with a negative index is absent: margin 0, no loss.  One with
  * an index >= candidates makes its margin and the loss NaN and has no
  * gradient.  grad receives d loss / d logp before that division and factor

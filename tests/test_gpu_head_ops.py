@@ -183,6 +183,17 @@ def test_propose_all_equal(fd):
             check_propose(fd, x.to(t), k, "id")
 
 
+def test_propose_mostly_zeros(fd):
+    """The bound falls on a logit of 0, which thousands share, in rows of
+    several stretches."""
+    x = torch.relu(torch.randn((1, 3, 300001), generator=gen(8), device="cuda") - 3)
+    x[0, 1] = torch.where(x[0, 1] > 0, x[0, 1], -0.0)
+    x[0, 2, 5:] = torch.where(x[0, 2, 5:] > 0, x[0, 2, 5:], -1e-30)
+    for t in (torch.float32, torch.bfloat16):
+        for k in (300, 1000, 6000):
+            check_propose(fd, x.to(t), k, "id")
+
+
 def test_propose_few_bounds_hold(fd):
     """Rows whose best logits the sample sees too often or not at all."""
     V = 262144

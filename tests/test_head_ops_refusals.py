@@ -1,8 +1,10 @@
 """What the C ABI of the model-side operators refuses, before anything is
 launched (no GPU needed), and the workspaces it asks for."""
 import ctypes
+import types
 
 import pytest
+import torch
 
 
 @pytest.fixture(scope="module")
@@ -149,6 +151,18 @@ def test_preference_too_many_pairs_refused(fd):
 def test_preference_smoothing_refused(fd, eps):
     p = preference(fd, label_smoothing=eps)
     assert fd._lib().ft_preference_loss_device(ctypes.byref(sequence(fd)), ctypes.byref(p), P, 1 << 40, None) == INVALID
+
+
+@pytest.mark.parametrize("beta", [float("inf"), float("-inf"), float("nan")])
+def test_preference_beta_refused(fd, beta):
+    p = preference(fd, beta=beta)
+    assert fd._lib().ft_preference_loss_device(ctypes.byref(sequence(fd)), ctypes.byref(p), P, 1 << 40, None) == INVALID
+
+
+def test_stream_of_another_device_refused(fd):
+    stream = types.SimpleNamespace(device_index=1)
+    with pytest.raises(ValueError, match="stream"):
+        fd._On(torch.device("cuda", 0), stream)
 
 
 def test_sequence_workspaces(fd):
