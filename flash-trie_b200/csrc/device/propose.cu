@@ -119,11 +119,14 @@ __device__ void block_range(Shared &sh, Key &low, Key &high) {
 
 // Keeps the entries of list[0, count) that are not below the returned key: at
 // least the k largest, and at most k + slack.  Radix selection, 11 bits a
-// pass, from the highest bit in which the entries differ.  count >= k.
-__device__ Key keep_largest(Shared &sh, Key *list, uint32_t count, uint32_t k, uint32_t slack) {
-  Key low = ~0ull, high = 0;
-  for (uint32_t i = threadIdx.x; i < count; i += kThreads) low = min(low, list[i]), high = max(high, list[i]);
-  block_range(sh, low, high);
+// pass, from the highest bit in which the entries differ.  count >= k.  With
+// low <= high at least k entries are known to lie in [low, high] and none above.
+__device__ Key keep_largest(Shared &sh, Key *list, uint32_t count, uint32_t k, uint32_t slack, Key low = ~0ull,
+                            Key high = 0) {
+  if (low > high) {
+    for (uint32_t i = threadIdx.x; i < count; i += kThreads) low = min(low, list[i]), high = max(high, list[i]);
+    block_range(sh, low, high);
+  }
   uint32_t need = k, sure = 0;
   for (;;) {
     const Key span = high - low;
@@ -162,14 +165,31 @@ __device__ Key keep_largest(Shared &sh, Key *list, uint32_t count, uint32_t k, u
     }
   }
   // In place: a round's entries are read before any is written, and no write
-  // goes beyond the entries read so far.
+  // goes beyond the entries read so far. A warp asks for its places at once.
+  constexpr int kRound = 4;
   __syncthreads();
   if (threadIdx.x == 0) sh.count = 0;
-  for (uint32_t i0 = 0; i0 < count; i0 += kThreads) {
-    const uint32_t i = i0 + threadIdx.x;
-    const Key x = i < count ? list[i] : 0;
+  for (uint32_t i0 = 0; i0 < count; i0 += kRound * kThreads) {
+    Key x[kRound];
+    uint32_t votes[kRound], all = 0;
+#pragma unroll
+    for (int q = 0; q < kRound; ++q) {
+      const uint32_t i = i0 + q * kThreads + threadIdx.x;
+      x[q] = i < count ? list[i] : 0;
+      votes[q] = __ballot_sync(~0u, i < count && x[q] >= low);
+      all += __popc(votes[q]);
+    }
     __syncthreads();
-    if (i < count && x >= low) list[atomicAdd(&sh.count, 1u)] = x;
+    const uint32_t lane = threadIdx.x & 31;
+    uint32_t at = 0;
+    if (lane == 0 && all) at = atomicAdd(&sh.count, all);
+    at = __shfl_sync(~0u, at, 0);
+#pragma unroll
+    for (int q = 0; q < kRound; ++q) {
+      if (votes[q] >> lane & 1) list[at + __popc(votes[q] & ((1u << lane) - 1))] = x[q];
+      at += __popc(votes[q]);
+    }
+    if (i0 + kRound * kThreads < count) __syncthreads();
   }
   __syncthreads();
   return low;
@@ -347,33 +367,59 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
   };
   {
-    constexpr int U = 8;  // 128 KB on their way per SM; 4 is 6% slower on f32, a third CTA per SM (spills) 30%
-    int64_t i = v0 + threadIdx.x;
-    for (; i + (U - 1) * kThreads < v1; i += U * kThreads) {
-      if (r.whole(i) && r.whole(i + (U - 1) * kThreads)) {
-        uint4 q[U];
+    // Four vectors of each thread on their way while four are added up; three
+    // are 3% slower, five no faster on bf16, and eight that are added up as soon
+    // as they are all there 7%: the CTAs of a row that fits on the GPU at once
+    // start together, and between the steps nothing would be on its way.
+    constexpr int U = 4;
+    constexpr int64_t kStep = U * kThreads;
+    // The vectors that the row's ends cut, one by one; [w0, w1) are whole.
+    const int64_t w0 = r.whole(v0) ? v0 : v0 + 1, w1 = v1 > w0 && !r.whole(v1 - 1) ? v1 - 1 : v1;
+    auto edge = [&](int64_t i) {
+      float v[N];
+      r.load_edge(i, v);
+      note(i, soft_add(s, v));
+    };
+    if (threadIdx.x == 0 && w0 > v0) edge(v0);
+    if (threadIdx.x == 32 && w1 < v1) edge(v1 - 1);
+    int64_t i = w0 + threadIdx.x;
+    auto fetch = [&](uint4 (&q)[U], int64_t at) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) q[u] = r.load_whole(i + u * kThreads);
-        float tops[U];
-        if (soft_add<T, U>(s, q, tops) > bound) {
+      for (int u = 0; u < U; ++u) q[u] = r.load_whole(at + u * kThreads);
+    };
+    auto take = [&](const uint4 (&q)[U], int64_t at) {
+      float tops[U];
+      if (soft_add<T, U>(s, q, tops) > bound) {
 #pragma unroll
-          for (int u = 0; u < U; ++u) note(i + u * kThreads, tops[u]);
+        for (int u = 0; u < U; ++u) note(at + u * kThreads, tops[u]);
+      }
+    };
+    auto full = [&](int64_t at) { return at + (U - 1) * kThreads < w1; };
+    if (full(i)) {
+      uint4 q[U], ahead[U];
+      fetch(q, i);
+      for (;;) {
+        if (!full(i + kStep)) {
+          take(q, i);
+          i += kStep;
+          break;
         }
-      } else {
-#pragma unroll 1
-        for (int u = 0; u < U; ++u) {
-          float v[N];
-          r.load_edge(i + u * kThreads, v);
-          note(i + u * kThreads, soft_add(s, v));
+        fetch(ahead, i + kStep);
+        take(q, i);
+        i += kStep;
+        if (!full(i + kStep)) {
+          take(ahead, i);
+          i += kStep;
+          break;
         }
+        fetch(q, i + kStep);
+        take(ahead, i);
+        i += kStep;
       }
     }
-    for (; i < v1; i += kThreads) {
+    for (; i < w1; i += kThreads) {
       float v[N];
-      if (r.whole(i))
-        unpack(r.load_whole(i), v, (const T *)nullptr);
-      else
-        r.load_edge(i, v);
+      unpack(r.load_whole(i), v, (const T *)nullptr);
       note(i, soft_add(s, v));
     }
   }
@@ -469,16 +515,21 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     __syncthreads();
   }
-  if (sampled && bound > kNegInf && count < k) {
+  bool bounded = sampled && bound > kNegInf;  // k entries above the bound are in the list
+  if (bounded && count < k) {
     careful(sh, list, r, 0, r.count(), k, p.cap);
     count = sh.count;
+    bounded = false;
   }
   if (threadIdx.x == 0) sh.sum = s;
   __syncthreads();
   s = sh.sum;
   if (!s.valid()) count = 0;
   if (count > k) {
-    keep_largest(sh, list, count, k, 0);
+    if (bounded)
+      keep_largest(sh, list, count, k, 0, (Key)ordered(bound) << 32, (Key)ordered(s.m) << 32 | 0xFFFFFFFFu);
+    else
+      keep_largest(sh, list, count, k, 0);
     count = sh.count;
   }
   // Ascending by (id) or by (falling logit, id).
