@@ -366,63 +366,11 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (at < p.hits) hit[at] = (uint32_t)(i - v0);
     }
   };
-  {
-    // Four vectors of each thread on their way while four are added up; three
-    // are 3% slower, five no faster on bf16, and eight that are added up as soon
-    // as they are all there 7%: the CTAs of a row that fits on the GPU at once
-    // start together, and between the steps nothing would be on its way.
-    constexpr int U = 4;
-    constexpr int64_t kStep = U * kThreads;
-    // The vectors that the row's ends cut, one by one; [w0, w1) are whole.
-    const int64_t w0 = r.whole(v0) ? v0 : v0 + 1, w1 = v1 > w0 && !r.whole(v1 - 1) ? v1 - 1 : v1;
-    auto edge = [&](int64_t i) {
-      float v[N];
-      r.load_edge(i, v);
-      note(i, soft_add(s, v));
-    };
-    if (threadIdx.x == 0 && w0 > v0) edge(v0);
-    if (threadIdx.x == 32 && w1 < v1) edge(v1 - 1);
-    int64_t i = w0 + threadIdx.x;
-    auto fetch = [&](uint4 (&q)[U], int64_t at) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) q[u] = r.load_whole(at + u * kThreads);
-    };
-    auto take = [&](const uint4 (&q)[U], int64_t at) {
-      float tops[U];
-      if (soft_add<T, U>(s, q, tops) > bound) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) note(at + u * kThreads, tops[u]);
-      }
-    };
-    auto full = [&](int64_t at) { return at + (U - 1) * kThreads < w1; };
-    if (full(i)) {
-      uint4 q[U], ahead[U];
-      fetch(q, i);
-      for (;;) {
-        if (!full(i + kStep)) {
-          take(q, i);
-          i += kStep;
-          break;
-        }
-        fetch(ahead, i + kStep);
-        take(q, i);
-        i += kStep;
-        if (!full(i + kStep)) {
-          take(ahead, i);
-          i += kStep;
-          break;
-        }
-        fetch(q, i + kStep);
-        take(ahead, i);
-        i += kStep;
-      }
-    }
-    for (; i < w1; i += kThreads) {
-      float v[N];
-      unpack(r.load_whole(i), v, (const T *)nullptr);
-      note(i, soft_add(s, v));
-    }
-  }
+  // Four vectors of each thread on their way while four are added up; three
+  // are 3% slower, five no faster on bf16, and eight that are added up as soon
+  // as they are all there 7%: the CTAs of a row that fits on the GPU at once
+  // start together, and between the steps nothing would be on its way.
+  soft_stream<T, kThreads, 4>(r, v0, v1, bound, s, note);
   s = soft_join_block<kThreads>(s, sh.sums);  // a barrier: all hits are noted
   const uint32_t hits = sh.hits;
   if (hits <= p.hits)

@@ -211,35 +211,61 @@ __device__ SoftSum soft_join_block(SoftSum s, SoftSum *smem /* [THREADS / 32] */
   return s;
 }
 
-// Adds the vectors [v0, v1) of a row to this thread's sum, U vectors of each
-// thread in flight at a time.
-template <typename T, int THREADS, int U>
-__device__ __forceinline__ void soft_stream(const RowVecs<T> &r, int64_t v0, int64_t v1, SoftSum &s) {
+// Adds the vectors [v0, v1) of a row to this thread's sum, U of them while U more
+// are on their way, and calls note(vector, its largest value) for those that may
+// hold something above `bound`.
+template <typename T, int THREADS, int U, typename Note>
+__device__ __forceinline__ void soft_stream(const RowVecs<T> &r, int64_t v0, int64_t v1, float bound, SoftSum &s, Note &&note) {
   constexpr int N = RowVecs<T>::N;
-  int64_t i = v0 + threadIdx.x;
-  for (; i + (U - 1) * THREADS < v1; i += U * THREADS) {
-    if (r.whole(i) && r.whole(i + (U - 1) * THREADS)) {
-      uint4 q[U];
+  constexpr int64_t kStep = U * THREADS;
+  // The vectors that the row's ends cut, one by one; [w0, w1) are whole.
+  const int64_t w0 = r.whole(v0) ? v0 : v0 + 1, w1 = v1 > w0 && !r.whole(v1 - 1) ? v1 - 1 : v1;
+  auto edge = [&](int64_t i) {
+    float v[N];
+    r.load_edge(i, v);
+    note(i, soft_add(s, v));
+  };
+  if (threadIdx.x == 0 && w0 > v0) edge(v0);
+  if (threadIdx.x == 32 && w1 < v1) edge(v1 - 1);
+  int64_t i = w0 + threadIdx.x;
+  auto full = [&](int64_t at) { return at + (U - 1) * THREADS < w1; };
+  auto fetch = [&](uint4 (&q)[U], int64_t at) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) q[u] = r.load_whole(i + u * THREADS);
-      float tops[U];
-      soft_add<T, U>(s, q, tops);
-    } else {
-#pragma unroll 1
-      for (int u = 0; u < U; ++u) {
-        float v[N];
-        r.load_edge(i + u * THREADS, v);
-        soft_add(s, v);
+    for (int u = 0; u < U; ++u) q[u] = r.load_whole(at + u * THREADS);
+  };
+  auto take = [&](const uint4 (&q)[U], int64_t at) {
+    float tops[U];
+    if (soft_add<T, U>(s, q, tops) > bound) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) note(at + u * THREADS, tops[u]);
+    }
+  };
+  if (full(i)) {
+    uint4 q[U], ahead[U];
+    fetch(q, i);
+    for (;;) {
+      if (!full(i + kStep)) {
+        take(q, i);
+        i += kStep;
+        break;
       }
+      fetch(ahead, i + kStep);
+      take(q, i);
+      i += kStep;
+      if (!full(i + kStep)) {
+        take(ahead, i);
+        i += kStep;
+        break;
+      }
+      fetch(q, i + kStep);
+      take(ahead, i);
+      i += kStep;
     }
   }
-  for (; i < v1; i += THREADS) {
+  for (; i < w1; i += THREADS) {
     float v[N];
-    if (r.whole(i))
-      unpack(r.load_whole(i), v, (const T *)nullptr);
-    else
-      r.load_edge(i, v);
-    soft_add(s, v);
+    unpack(r.load_whole(i), v, (const T *)nullptr);
+    note(i, soft_add(s, v));
   }
 }
 
