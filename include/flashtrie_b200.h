@@ -299,7 +299,7 @@ int ft_propose_device(const ft_propose_args *args, void *workspace, uint64_t wor
  * tokens and lengths have the layout of the search's results (out_tok,
  * out_len with out_capacity = candidates).  Length 0 gives 0; a length
  * outside [0, num_outpos] gives NaN and takes no part in gradients; tokens
- * behind a length are not read.  A token id >= vocab counts as a logit of
+ * behind a length do not matter.  A token id >= vocab counts as a logit of
  * -inf, and so does every token of a position whose logits are all -inf; such
  * a position has no gradient.  candidates is at most 8192.  `stats` receives
  * (maximum, sum of exponentials) of every row, which the gradient reads.

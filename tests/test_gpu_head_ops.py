@@ -588,7 +588,7 @@ def test_preference_far_margins(fd):
         loss, margin = fd.preference_loss(x, toks, lens, ref, *pair, beta=0.1)
         (dx,) = torch.autograd.grad(loss, x)
         if far > 0:
-            assert float(loss) == 0.0 and not bool(dx.any())
+            assert float(loss.detach()) == 0.0 and not bool(dx.any())
         else:
             assert abs(float(loss) + float(margin)) <= 2 * U * abs(float(margin)) and float(dx.abs().max()) > 0.05
 
