@@ -125,6 +125,7 @@ __device__ uint32_t block_exclusive(uint32_t x, uint32_t *total, uint32_t *sm /*
 
 // One CTA of 1024 threads: the requests in order of (adapter, request), their
 // groups and columns.  The sort key is unique, so the order is always the same.
+// Latency: 6.7 us for 8 requests, 9 for 64 of 20 tokens.
 __global__ void __launch_bounds__(1024) order_kernel(const int32_t *ids, uint32_t n, uint32_t L, uint32_t num_adapters,
                                                      uint32_t slots, uint32_t tile_t, Sorted o) {
   extern __shared__ unsigned long long key[];  // [slots], then u32 [slots] group of a position, u32 [slots] its start
@@ -198,7 +199,10 @@ constexpr int kShrinkTokens = 4, kShrinkRows = 4;
 // u of up to four tokens of a request: a warp takes four low-rank rows, its
 // lanes the inner dimension. The sorted form also moves the tokens to their
 // columns and splits u into 16-bit parts, laid out as the products read them,
-// the parts of eight columns next to one another.
+// the parts of eight columns next to one another. Tokens four to a CTA, so that
+// a few of them spread over many SMs: latency, 2.7 us for 8 tokens of D = 512
+// and 5.8 for 128 of 768; 20 us for 1280 tokens of 2048 and rank 64, each CTA
+// reading its adapter's rows from L2.
 template <typename T, bool kSorted>
 __global__ void __launch_bounds__(256) shrink_kernel(ft_adapter_args a, float *u, Sorted o) {
   const uint32_t per = (a.num_outpos + kShrinkTokens - 1) / kShrinkTokens;
@@ -293,7 +297,8 @@ constexpr int kExpandThreads = 256, kExpandRows = 4, kExpandTokens = 4;
 // The direct form's low-rank part: four vocabulary entries per thread, 256
 // apart, for the tokens of one request. What costs here is getting to the rows
 // of B, so that four are on their way at once; rows staged through shared
-// memory in whole lines came out three times slower.
+// memory in whole lines came out three times slower. 7.3 us for 37 single
+// tokens with 40 adapters by 32000 of rank 16 (38 MB of rows, 5.2 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(kExpandThreads) expand_kernel(ft_adapter_args a, const float *u, float *delta) {
   sm100::launch_next();
@@ -437,6 +442,15 @@ __device__ __forceinline__ bool walk_tile(const Walk &k, bool sorted, const Grou
 
 // Persistent, one CTA per SM.  Tiles that share a stretch of the weight are
 // neighbours in the order, so that it comes from DRAM once.
+//
+// Few tokens: bound by the weight's bytes, 688 us for 20 tokens by 2.2M x 1024
+// bf16 (4.6 GB, 6.7 TB/s), 156 us for 128 by 500k x 768 with f32 logits (1.02
+// GB, 6.6 TB/s) and 179 with eight adapters.  Full batches: bound by what an SM
+// takes in and by the power limit.  1280 tokens by 500k x 2048 with 16 adapters
+// of rank 64 take 2.39 ms (1130 TFLOP/s of useful products).  By 100k, the shared
+// product alone takes 379 us (1384 TFLOP/s) and with adapters 470 to 490: the
+// padded columns make a sixth tile of tokens, which loads the weight once more
+// (a seventh of the time), the rest are the adapters' rows and values.
 template <typename T, typename O, bool kSorted>
 __global__ void __launch_bounds__(kThreads, 1)
     logits_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_h,

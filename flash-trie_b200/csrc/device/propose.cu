@@ -10,14 +10,19 @@
 //
 // The logits are read once.  A row is cut into stretches, a CTA each.  A
 // sample spread over the row gives a bound that a little more than k entries
-// should pass; the CTA streams its stretch, adds to the
-// softmax sum and notes the vectors in which something passes the bound (noting
-// takes a few instructions, taking the entries out at once a fifth of the
-// stream's time); then it fetches those again and keeps what passes.  The CTA that
-// ends last in its row joins the sums, selects the k largest of what all have
-// kept, and sorts them.  The bound is a guess only: a stretch that keeps more
-// than fits is read again with a bound that rises (`careful`), and a row that
-// kept fewer than k is read again by its last CTA without one.
+// should pass; the CTA streams its stretch, adds to the softmax sum and notes
+// the vectors in which something passes the bound (a few instructions; taking
+// the entries out at once would cost a fifth of the stream's time); then it
+// fetches those again and keeps what passes.  The CTA that ends last in its row
+// joins the sums, selects the k largest of what all have kept, and sorts them.
+// The bound is a guess only: a stretch that keeps more than fits is read again
+// with a bound that rises (`careful`), and a row that kept fewer than k is read
+// again by its last CTA without one.
+//
+// Large batches are bound by the logits' bytes: 92 us for 256 rows of 500009 f32
+// (512 MB, 5.6 TB/s), k 256, a CTA per row.  One request is bound by latency
+// around its stream: 47.5 us for 20 rows of 2.2M bf16 (88 MB, 13.5 us at the
+// copy rate), k 1000; 14.5 us for 8 rows of 32000 f32, k 64.
 #include <algorithm>
 #include <string>
 
