@@ -13,11 +13,13 @@
 // The low-rank part has two forms.  "Sorted": the tokens are put in order of
 // their adapters, each adapter's at a multiple of 16 columns, and every group
 // adds its u B^T to its own columns with further tensor products; u goes in as
-// two or three 16-bit parts, so that no more than 2^-18 of it is lost (2^-27
-// for f32 logits).  No column is shared, so an adapter with infinities reaches
-// no other one's requests.  "Direct": the tokens stay as they are, a kernel of
-// its own makes the low-rank part in 32 bits and the epilogue adds it, for
-// batches whose groups are so small that padding them would cost more.
+// 16-bit parts: a bf16 part leaves at most 2^-8 of its power of two, a value of
+// the power 2^-9 or below for the next, so that two parts lose 2^-17 and the
+// three for f32 logits 2^-26; two f16 parts lose 2^-23, or 2^-25 absolute.  No
+// column is shared, so an adapter with infinities reaches no other one's
+// requests.  "Direct": the tokens stay as they are, a kernel of its own makes
+// the low-rank part in 32 bits and the epilogue adds it, for batches whose
+// groups are so small that padding them would cost more.
 #include <algorithm>
 #include <string>
 

@@ -242,7 +242,7 @@ int ft_tbs_batch_device_noalloc(ft_trie *trie, const ft_device_batch *batch,
  * lora_a and lora_b are dtype (bf16 or f16), out is out_dtype (the same type,
  * or f32); all five start on 16-byte boundaries.  dim and rank are multiples
  * of 8, rank at most 256.  With f16 operands scale * (hidden lora_a) must stay
- * within f16's range (65504), and is kept to 2^-25 absolute or better.  An
+ * within f16's range (65504); 2^-23 of it is lost, or 2^-25 absolute.  An
  * infinite one, or an infinity in lora_b, makes the logits that it enters NaN
  * or infinite.  out overlaps none of the inputs.  num_adapters = 0: adapter_ids, lora_a, lora_b and
  * scale are not read.  scale may be NULL (1 for every adapter).  At most
