@@ -142,9 +142,9 @@ __device__ double2 block_sum(double2 v, double2 *sm /* [kPairThreads / 32] */) {
   return s;
 }
 
-// Sums of floats that do not depend on the order of the additions: integers in
-// units of a power of two that leaves room for `terms` of them of magnitude
-// below 2^exponent.  For a thousand terms a unit is 2^-51 of that magnitude.
+// Sums that do not depend on the order of the additions: integers in units of a
+// power of two that leaves room for `terms` of them of magnitude below
+// 2^exponent.  For a thousand terms a unit is 2^-51 of that magnitude.
 struct FixedSum {
   double up, down;
   __device__ FixedSum(int exponent, uint32_t terms) {
@@ -155,6 +155,13 @@ struct FixedSum {
   __device__ unsigned long long of(double x) const { return (unsigned long long)__double2ll_rn(x * up); }
   __device__ double value(unsigned long long s) const { return (double)(long long)s * down; }
 };
+
+// The power of two above a weight's magnitude, as an integer that compares as
+// the magnitudes do: |w| < 2^(power_above(w) - 1022).  Weights below 2^-300
+// count as that; no f32 holds them.
+__device__ __forceinline__ uint32_t power_above(double w) {
+  return max((uint32_t)__double2hiint(w) >> 20 & 0x7FFu, 1022u - 300u);
+}
 
 // Adds to a 64-bit sum in shared memory. There, the hardware adds 32 bits at
 // once but 64 only in a loop that tries again whenever another thread was
@@ -169,41 +176,53 @@ __device__ __forceinline__ void add_shared(unsigned long long *sum, unsigned lon
 
 // The pairs of one request per CTA: margins, this request's loss and pair
 // count, and each candidate's gradient, added up in shared memory as integers
-// so that it is the same in any order (the weights are below |beta|).  The CTA
-// that ends last adds up the requests.  Latency of looks one after the other:
-// 9.4 us for 1000 pairs, 7.7 for 8.
+// so that it is the same in any order.  Weights fall with e^-margin, so that
+// each candidate's sum has a unit of its own, by its largest weight: the first
+// pass finds that and the second adds (a thread keeps its first pair's weight,
+// those of further pairs are worked out again).  The CTA that ends last adds up
+// the requests.  Latency of looks one after the other: 9.4 us for 1000 pairs,
+// 7.7 for 8.
 __global__ void __launch_bounds__(kPairThreads)
     pair_kernel(ft_preference_args p, uint32_t n, uint32_t C, const double *logp64, double2 *part, uint32_t *ticket) {
-  extern __shared__ unsigned long long acc[];  // [C], then C bits: the candidate is in a pair without a margin
-  uint32_t *broken = reinterpret_cast<uint32_t *>(acc + C);
+  // [C] sums, u32 [C] the power above each one's largest weight (0: no pair),
+  // then C bits: the candidate is in a pair without a margin.
+  extern __shared__ unsigned long long acc[];
+  uint32_t *top = reinterpret_cast<uint32_t *>(acc + C), *broken = top + C;
   __shared__ double2 sm[kPairThreads / 32];
   __shared__ bool last;
   const uint64_t req = blockIdx.x;
   const double *lp = logp64 + req * C;
   const float *ref = p.ref_logp + req * C;
-  const FixedSum fix(p.beta != 0.0f ? ilogb((double)p.beta) + 1 : 0, 2 * p.pairs);
-  for (uint32_t j = threadIdx.x; j < C; j += kPairThreads) acc[j] = 0;
+  const int32_t *chosen = p.chosen + req * p.pairs, *rejected = p.rejected + req * p.pairs;
+  const double beta = p.beta, e = p.label_smoothing;
+  auto margin_of = [&](int32_t c, int32_t r) { return beta * ((lp[c] - (double)ref[c]) - (lp[r] - (double)ref[r])); };
+  auto weight_of = [&](double z, double t /* exp(-|z|) */) {
+    const double big = 1.0 / (1.0 + t), small = t / (1.0 + t);  // sigmoids of |z| and -|z|
+    return beta * (e * (z >= 0 ? big : small) - (1.0 - e) * (z >= 0 ? small : big));
+  };
+  auto there = [&](int32_t c, int32_t r) { return c >= 0 && r >= 0 && (uint32_t)c < C && (uint32_t)r < C; };
+  for (uint32_t j = threadIdx.x; j < C; j += kPairThreads) acc[j] = 0, top[j] = 0;
   for (uint32_t j = threadIdx.x; j < (C + 31) / 32; j += kPairThreads) broken[j] = 0;
   __syncthreads();
-  double loss = 0.0, count = 0.0;
+  double loss = 0.0, count = 0.0, kept = 0.0;
   for (uint32_t q = threadIdx.x; q < p.pairs; q += kPairThreads) {
-    const int32_t c = p.chosen[req * p.pairs + q], r = p.rejected[req * p.pairs + q];
+    const int32_t c = chosen[q], r = rejected[q];
     float margin = 0.0f;
     if (c >= 0 && r >= 0) {
       count += 1.0;
-      if ((uint32_t)c < C && (uint32_t)r < C) {
-        const double z = (double)p.beta * ((lp[c] - (double)ref[c]) - (lp[r] - (double)ref[r]));
-        const double e = p.label_smoothing, t = exp(-fabs(z)), soft = log1p(t);
+      if (there(c, r)) {
+        const double z = margin_of(c, r);
+        const double t = exp(-fabs(z)), soft = log1p(t);
         const double pos = soft + (z < 0 ? -z : 0.0), neg = soft + (z > 0 ? z : 0.0);
-        const double big = 1.0 / (1.0 + t), small = t / (1.0 + t);  // sigmoids of |z| and -|z|
         // A weight of zero takes its side away whatever that side's value.
         loss += (e < 1.0 ? (1.0 - e) * pos : 0.0) + (e > 0.0 ? e * neg : 0.0) + (z != z ? z : 0.0);
         margin = (float)z;
         if (z == z) {
-          const double w = (double)p.beta * (e * (z >= 0 ? big : small) - (1.0 - e) * (z >= 0 ? small : big));
-          const unsigned long long u = fix.of(w);
-          add_shared(&acc[c], u);
-          add_shared(&acc[r], 0ull - u);
+          const double w = weight_of(z, t);
+          const uint32_t power = power_above(w);
+          atomicMax(&top[c], power);
+          atomicMax(&top[r], power);
+          if (q == threadIdx.x) kept = w;
         } else {
           atomicOr(&broken[(uint32_t)c / 32], 1u << (c % 32));
           atomicOr(&broken[(uint32_t)r / 32], 1u << (r % 32));
@@ -215,9 +234,26 @@ __global__ void __launch_bounds__(kPairThreads)
     }
     p.margin[req * p.pairs + q] = margin;
   }
-  const double2 sums = block_sum(make_double2(loss, count), sm);  // its barriers make acc complete
-  for (uint32_t j = threadIdx.x; j < C; j += kPairThreads)
-    p.grad[req * C + j] = broken[j / 32] >> (j % 32) & 1 ? __int_as_float(0x7FC00000) : (float)fix.value(acc[j]);
+  const double2 sums = block_sum(make_double2(loss, count), sm);  // its barriers make top and broken complete
+  const uint32_t terms = 2 * (uint32_t)sums.y;
+  for (uint32_t q = threadIdx.x; q < p.pairs; q += kPairThreads) {
+    const int32_t c = chosen[q], r = rejected[q];
+    if (!there(c, r)) continue;
+    double w = kept;
+    if (q != threadIdx.x) {
+      const double z = margin_of(c, r);
+      if (z != z) continue;
+      w = weight_of(z, exp(-fabs(z)));
+    }
+    if (w == 0.0) continue;
+    add_shared(&acc[c], FixedSum((int)top[c] - 1022, terms).of(w));
+    add_shared(&acc[r], FixedSum((int)top[r] - 1022, terms).of(-w));
+  }
+  __syncthreads();
+  for (uint32_t j = threadIdx.x; j < C; j += kPairThreads) {
+    const float g = top[j] ? (float)FixedSum((int)top[j] - 1022, terms).value(acc[j]) : 0.0f;
+    p.grad[req * C + j] = broken[j / 32] >> (j % 32) & 1 ? __int_as_float(0x7FC00000) : g;
+  }
   if (threadIdx.x == 0) {
     part[req] = sums;
     __threadfence();
@@ -597,8 +633,8 @@ void preference_loss_device(const ft_sequence_args &a, const ft_preference_args 
   double *lp = reinterpret_cast<double *>(w + l.lp);
   uint32_t *ticket = reinterpret_cast<uint32_t *>(w + l.ticket);
   scores(a, w, lp, ticket, stream);
-  const size_t smem = 8ull * a.candidates + 4 * ((a.candidates + 31) / 32);
-  allow_shared(pair_kernel, 8 * kMaxCandidates + kMaxCandidates / 8);
+  const size_t smem = 12ull * a.candidates + 4 * ((a.candidates + 31) / 32);
+  allow_shared(pair_kernel, 12 * kMaxCandidates + kMaxCandidates / 8);
   pair_kernel<<<a.n, kPairThreads, smem, stream>>>(p, a.n, a.candidates, lp, reinterpret_cast<double2 *>(w + l.part),
                                                    ticket);
   CUDA_TRY(cudaGetLastError());
