@@ -279,15 +279,18 @@ __global__ void __launch_bounds__(kPairThreads)
 // One CTA per row: W, and the summed weight of each distinct token of the live
 // candidates.  The tokens meet in a hash table in shared memory (at most half
 // full) whose sums are integers, so that they are the same in any order; the
-// list's order is not, and nothing depends on it.  A weight that is not finite
-// makes W NaN, and with it the row's gradient.  Latency: 5.9 us for 48 rows of
-// 1000 candidates, 4.1 for 128 of 10.
+// list's order is not, and nothing depends on it.  Each token's sum has a unit
+// of its own, by the exponent of its largest weight, which the first pass finds.
+// A weight that is not finite makes W NaN, and with it the row's gradient.
+// Latency: 5.9 us for 48 rows of 1000 candidates, 4.1 for 128 of 10.
 __global__ void __launch_bounds__(kPlanThreads)
     scatter_plan_kernel(const uint32_t *tokens, const int32_t *lengths, const SoftSum *stats, const float *grad,
                         const float *factor, const float *upstream, uint32_t vocab, uint32_t L, uint32_t C,
                         uint32_t slots, uint32_t *out_tok, float *out_w, uint32_t *out_n, float *out_total) {
-  extern __shared__ unsigned long long acc[];  // [slots], then u32 [slots] tokens
+  // [slots] sums, which begin as the exponent; u32 [slots] tokens; u8 [slots] exponents.
+  extern __shared__ unsigned long long acc[];
   uint32_t *key = reinterpret_cast<uint32_t *>(acc + slots);
+  uint8_t *power = reinterpret_cast<uint8_t *>(key + slots);
   __shared__ double2 sm[32];
   __shared__ uint32_t found, largest;
   const uint64_t row = blockIdx.x, req = row / L;
@@ -325,18 +328,29 @@ __global__ void __launch_bounds__(kPlanThreads)
     if (threadIdx.x == 0) out_n[row] = 0, out_total[row] = (float)(total * scale);
     return;
   }
-  const FixedSum fix(ilogbf(__uint_as_float(top)) + 1, C);
+  // A weight of exponent field e is below 2^(e - 126).  token[q] becomes its slot.
+  auto fixed = [&](uint32_t e) { return FixedSum((int)e - 126, C); };
 #pragma unroll
   for (int q = 0; q < kMost; ++q) {
     const uint32_t t = token[q];
+    token[q] = 0xFFFFFFFFu;
     if (t >= vocab) continue;
     uint32_t at = (t * 2654435761u) >> (32 - __popc(slots - 1));
     for (uint32_t i = 0; i < slots; ++i, at = (at + 1) & (slots - 1)) {
       const uint32_t was = atomicCAS(&key[at], 0xFFFFFFFFu, t);
       if (was == 0xFFFFFFFFu || was == t) break;
     }
-    add_shared(&acc[at], fix.of(weight[q]));
+    token[q] = at;
+    atomicMax(reinterpret_cast<uint32_t *>(&acc[at]), __float_as_uint(weight[q]) >> 23 & 0xFFu);
   }
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < kMost; ++q)
+    if (token[q] < slots) power[token[q]] = (uint8_t)acc[token[q]];  // one value, whoever writes it
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < kMost; ++q)
+    if (token[q] < slots) add_shared(&acc[token[q]], fixed(power[token[q]]).of(weight[q]));
   __syncthreads();
   for (uint32_t i0 = 0; i0 < slots; i0 += blockDim.x) {  // a warp asks for its places at once
     const uint32_t i = i0 + threadIdx.x;
@@ -347,7 +361,7 @@ __global__ void __launch_bounds__(kPlanThreads)
     at = __shfl_sync(~0u, at, 0) + __popc(votes & ((1u << lane) - 1));
     if (has) {
       out_tok[row * C + at] = key[i];
-      out_w[row * C + at] = (float)(fix.value(acc[i]) * scale);
+      out_w[row * C + at] = (float)(fixed(power[i]).value(acc[i] - power[i]) * scale);
     }
   }
   __syncthreads();
@@ -585,8 +599,8 @@ void sequence_grad_device(const ft_sequence_args &a, const float *grad, const fl
   uint32_t slots = 32;
   while (slots < 2 * a.candidates) slots <<= 1;
   const uint32_t threads = std::min<uint32_t>(kPlanThreads, (a.candidates + 31) / 32 * 32);
-  const size_t smem = 12ull * slots;
-  allow_shared(scatter_plan_kernel, 12 * 2 * kMaxCandidates);
+  const size_t smem = 13ull * slots;
+  allow_shared(scatter_plan_kernel, 13 * 2 * kMaxCandidates);
   scatter_plan_kernel<<<(unsigned)p.rows, threads, smem, stream>>>(a.tokens, a.lengths, stats, grad, factor, upstream,
                                                                    a.vocab, a.num_outpos, a.candidates, slots, tok,
                                                                    tok_w, cnt, total);
