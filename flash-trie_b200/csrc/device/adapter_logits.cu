@@ -15,7 +15,10 @@
 // adds its u B^T to its own columns with further tensor products; u goes in as
 // 16-bit parts: a bf16 part leaves at most 2^-8 of its power of two, a value of
 // the power 2^-9 or below for the next, so that two parts lose 2^-17 and the
-// three for f32 logits 2^-26; two f16 parts lose 2^-23, or 2^-25 absolute.  No
+// three for f32 logits 2^-26; two f16 parts lose 2^-23, or 2^-25 absolute.  A
+// token whose largest value is beyond the type's range, or so small that 2^-25
+// would show, takes no part in these products: its values stay in 32 bits and
+// the epilogue adds its low-rank part, slowly but the same as "direct" does.  No
 // column is shared, so an adapter with infinities reaches no other one's
 // requests.  "Direct": the tokens stay as they are, a kernel of its own makes
 // the low-rank part in 32 bits and the epilogue adds it, for batches whose
@@ -93,16 +96,35 @@ struct Sorted {
   uint32_t *tile_first;  // first group of each tile of tokens
   Group *tile_groups;    // [tiles][kTileGroups]: the groups with columns in a tile, then one that begins nowhere
   uint32_t *req_col;     // first column of each request
-  int32_t *col_token;    // token of a column; -1 padding; -2 - token: of a request whose adapter does not exist
+  // Token of a column, with kWide if its low-rank values are in `wide` alone;
+  // -1 padding; -2 - token: of a request whose adapter does not exist.
+  int32_t *col_token;
+  float *wide;           // [tokens][rank], written for tokens with kWide
   void *hidden;          // [columns][dim]
   uint8_t *u;            // [rank / width][columns / 8][parts][8 columns][width], swizzled as in shared memory
   uint32_t columns;      // upper bound, a multiple of 16
   uint32_t parts;
   uint32_t width;        // low-rank rows that a product's operands hold side by side: 16, 32 or 64
   // One request: its tokens are in order as they are. There are no tables and
-  // no moved tokens; only u is written.
+  // no moved tokens; only u and, where the request has an adapter, its tokens'
+  // entries of col_token are written.
   bool single;
 };
+
+constexpr int32_t kWide = 1 << 24;  // above any token's number
+constexpr uint64_t kMaxTokens = 0x3FFFFF;
+static_assert(kMaxTokens < kWide, "a token's number and the flag share a word");
+
+// Whether the 16-bit parts hold the low-rank values of a token, by the largest
+// magnitude among them.  f16 ends at 65504, and below 2^-8 the 2^-25 that its
+// two parts leave is more than 2^-17 of the largest.  bf16 has f32's range;
+// there the parts' own range ends.
+__device__ __forceinline__ bool parts_hold(float most, const __half *) {
+  return most == 0.0f || (most >= 0x1p-8f && most <= 65504.0f);
+}
+__device__ __forceinline__ bool parts_hold(float most, const __nv_bfloat16 *) {
+  return most == 0.0f || (most >= 0x1p-100f && most <= 0x1p+127f);
+}
 
 // Sum over the items of the threads before this one, and over all.
 __device__ uint32_t block_exclusive(uint32_t x, uint32_t *total, uint32_t *sm /* [32] */) {
@@ -201,7 +223,9 @@ constexpr int kShrinkTokens = 4, kShrinkRows = 4;
 // u of up to four tokens of a request: a warp takes four low-rank rows, its
 // lanes the inner dimension. The sorted form also moves the tokens to their
 // columns and splits u into 16-bit parts, laid out as the products read them,
-// the parts of eight columns next to one another. Tokens four to a CTA, so that
+// the parts of eight columns next to one another; the values meet in shared
+// memory before, where each token's largest decides whether parts hold them.
+// Tokens four to a CTA, so that
 // a few of them spread over many SMs: latency, 2.7 us for 8 tokens of D = 512
 // and 5.8 for 128 of 768; 20 us for 1280 tokens of 2048 and rank 64, each CTA
 // reading its adapter's rows from L2.
@@ -216,6 +240,8 @@ __global__ void __launch_bounds__(256) shrink_kernel(ft_adapter_args a, float *u
   const T *h = static_cast<const T *>(a.hidden) + tok * a.dim;
   const uint32_t lane = threadIdx.x & 31;
   uint32_t col = 0;
+  __shared__ float low[kSorted ? kShrinkTokens : 1][kSorted ? kMaxRank : 1];
+  __shared__ bool wide[kShrinkTokens];
   sm100::launch_next();
   if (kSorted && o.single) {
     col = l0;
@@ -225,11 +251,11 @@ __global__ void __launch_bounds__(256) shrink_kernel(ft_adapter_args a, float *u
     uint4 *to = reinterpret_cast<uint4 *>(static_cast<T *>(o.hidden) + (uint64_t)col * a.dim);
     const uint4 *from = reinterpret_cast<const uint4 *>(h);
     for (uint32_t i = threadIdx.x; i < count * (a.dim / 8); i += 256) to[i] = from[i];
-    if (threadIdx.x < count) {
+    if (!has) {  // its columns take no part in any group's products
       const int32_t t = (int32_t)(tok + threadIdx.x);
-      o.col_token[col + threadIdx.x] = has || id == -1 ? t : -2 - t;
+      if (threadIdx.x < count) o.col_token[col + threadIdx.x] = id == -1 ? t : -2 - t;
+      return;
     }
-    if (!has) return;  // its columns take no part in any group's products
   }
   const float scale = has && a.scale ? a.scale[id] : 1.0f;
   // Rows up to the next multiple of 16 exist as zeros in the sorted form.
@@ -275,21 +301,40 @@ __global__ void __launch_bounds__(256) shrink_kernel(ft_adapter_args a, float *u
 #pragma unroll
         for (int y = 0; y < kShrinkTokens; ++y)
           if (i == x && q == y) v = s[x][y];
-      if (!kSorted) {
+      if (kSorted)
+        low[q][r + i] = v;
+      else
         u[(tok + q) * a.rank + r + i] = v;
-      } else {
-        const uint32_t c = col + q, row = o.width * 2;
-        uint8_t *at = o.u + ((uint64_t)((r + i) / o.width) * (o.columns / 8) + c / 8) * o.parts * 8 * row +
-                      sm100::swizzled(c % 8 * row + (r + i) % o.width * 2, row);
-        for (uint32_t part = 0; part < o.parts; ++part) {
-          T x;
-          from_f32(v, x);
-          *reinterpret_cast<T *>(at + part * 8 * row) = x;
-          // What is left for the next part; nothing behind an infinity.
-          const float back = to_f32(x);
-          v = fabsf(back) < -kNegInf ? v - back : 0.0f;
-        }
-      }
+    }
+  }
+  if (!kSorted) return;
+  __syncthreads();
+  if (const uint32_t q = threadIdx.x >> 5; q < count) {
+    float most = 0.0f;
+    for (uint32_t r = lane; r < a.rank; r += 32) most = fmaxf(most, fabsf(low[q][r]));
+#pragma unroll
+    for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
+    if (lane == 0) {
+      wide[q] = !parts_hold(most, (const T *)nullptr);
+      o.col_token[col + q] = (int32_t)(tok + q) | (wide[q] ? kWide : 0);
+    }
+  }
+  __syncthreads();
+  const uint32_t row = o.width * 2;
+  for (uint32_t i = threadIdx.x; i < count * rows; i += 256) {
+    const uint32_t q = i / rows, r = i % rows, c = col + q;
+    float v = low[q][r];
+    if (wide[q]) {
+      if (r < a.rank) o.wide[(tok + q) * a.rank + r] = v;
+      v = 0.0f;
+    }
+    uint8_t *at = o.u + ((uint64_t)(r / o.width) * (o.columns / 8) + c / 8) * o.parts * 8 * row +
+                  sm100::swizzled(c % 8 * row + r % o.width * 2, row);
+    for (uint32_t part = 0; part < o.parts; ++part) {
+      T x;
+      from_f32(v, x);
+      *reinterpret_cast<T *>(at + part * 8 * row) = x;
+      v -= to_f32(x);  // what is left for the next part
     }
   }
 }
@@ -367,7 +412,7 @@ struct alignas(16) LogitsShared {
   // (in bytes; negative: it has none), and which columns' logits are NaN.
   int64_t begin[2][kMaxTileT];
   uint32_t wrong[2][kMaxTileT / 32];
-  uint32_t more[2][kMaxTileT / 32];  // direct form: which columns' have a low-rank part
+  uint32_t more[2][kMaxTileT / 32];  // which columns' low-rank part the epilogue adds
   uint32_t tmem, gave_up;
 };
 
@@ -397,6 +442,19 @@ LogitsPlan plan_logits(const ft_adapter_args &a, uint32_t columns, uint32_t part
   return p;
 }
 size_t logits_smem(const LogitsPlan &p) { return 1024 + (size_t)p.stages * p.stage; }
+
+// sum_r u[r] b[r] of a token whose low-rank values are in 32 bits alone.
+template <typename T>
+__device__ __noinline__ float wide_part(const T *b, const float *u, uint32_t rank) {
+  float s = 0.0f;
+  for (uint32_t r = 0; r < rank; r += 8) {
+    float w[8];
+    unpack8<T>(__ldg(reinterpret_cast<const uint4 *>(b + r)), w);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = fmaf(__ldcg(u + r + e), w[e], s);
+  }
+  return s;
+}
 
 // What a walk reads again and again, in registers.
 struct Walk {
@@ -488,6 +546,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const Walk walk{p.tile_t, p.stage, p.group_rows, p.group_column, p.group_most, o.width,
                   kSorted ? (a.rank + o.width - 1) / o.width : 0, (a.dim + kTileD - 1) / kTileD};
   const int32_t only = kSorted && o.single ? a.adapter_ids[0] : -1;
+  const bool single_low = kSorted && o.single && (uint32_t)only < a.num_adapters;
 
   // A tile's groups, one a lane, are fetched while the tile before is under
   // way: a look into global memory takes microseconds when the memory is busy,
@@ -638,6 +697,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t split = p.split, apart = p.acc, set = halves * split * apart;
     const uint32_t mine = tmem + half * split * apart + ((warp & 3) << 21);
     uint8_t *const logits = static_cast<uint8_t *>(a.out);
+    if (single_low) wait_for_previous();  // col_token
     for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
       const uint32_t b = n % buffers, t0 = tile % tiles_t * tile_t;
       const uint32_t v = tile / tiles_t * halves * kTileV + row;
@@ -650,16 +710,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (c < count) {
           token = (int32_t)(t0 + c);
           if (kSorted && o.single) {
-            bad = (uint32_t)only >= a.num_adapters && only != -1;
-            if (t0 + c >= a.num_outpos) token = -1;
+            bad = !single_low && only != -1;
+            if (t0 + c >= a.num_outpos)
+              token = -1;
+            else if (single_low)
+              token = __ldcg(&o.col_token[t0 + c]);
           } else if (kSorted) {
-            token = o.col_token[t0 + c];
+            token = __ldcg(&o.col_token[t0 + c]);
             bad = token < -1;
             if (bad) token = -2 - token;
           } else if (delta) {
             const int32_t id = a.adapter_ids[token / a.num_outpos];
             more = (uint32_t)id < a.num_adapters;
             bad = !more && id != -1;
+          }
+          if (kSorted && token >= kWide) {
+            token -= kWide;
+            more = true;
           }
         }
         sh.begin[n & 1][c] = token < 0 ? -1 : (int64_t)token * pitch;
@@ -699,6 +766,20 @@ __global__ void __launch_bounds__(kThreads, 1)
             add[e] = live && (any >> e & 1) ? __ldg(&delta[(uint64_t)(t0 + c0 + e) * vocab + v]) : 0.0f;
 #pragma unroll
           for (int e = 0; e < 16; ++e) acc[e] = __float_as_uint(__uint_as_float(acc[e]) + add[e]);
+        }
+        if (kSorted) {
+          const uint32_t any = sh.more[n & 1][c0 / 32] >> (c0 % 32) & 0xFFFF;
+          if (any && live) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (any >> e & 1) {
+                const uint32_t token = (uint32_t)(begin[c0 + e] / pitch);
+                const int32_t id = o.single ? only : a.adapter_ids[token / a.num_outpos];
+                acc[e] = __float_as_uint(__uint_as_float(acc[e]) +
+                                         wide_part(static_cast<const T *>(a.lora_b) + ((uint64_t)id * vocab + v) * a.rank,
+                                                   o.wide + (uint64_t)token * a.rank, a.rank));
+              }
+          }
         }
         if (wrong) {
 #pragma unroll
@@ -817,7 +898,7 @@ void check_adapter(const ft_adapter_args &a) {
     throw InvalidArgument("adapter_logits: rank must be a multiple of 8 in [8, 256]");
   if (a.num_adapters > kMaxAdapters) throw InvalidArgument("adapter_logits: at most 65536 adapters");
   // Token and vocabulary coordinates of a tile are 32-bit.
-  if ((uint64_t)a.n * a.num_outpos > 0x3FFFFF || a.vocab > 0x3FFFFF00u || a.dim > 0xFFFFFF ||
+  if ((uint64_t)a.n * a.num_outpos > kMaxTokens || a.vocab > 0x3FFFFF00u || a.dim > 0xFFFFFF ||
       (uint64_t)(a.vocab / kTileV + 1) * ((uint64_t)a.n * a.num_outpos / 16 + 1) > 0x7FFFFFFF ||
       (uint64_t)(a.vocab / kExpandThreads + 1) * a.n > 0x7FFFFFFF)
     throw InvalidArgument("adapter_logits: too many tokens or too large a vocabulary");
@@ -829,7 +910,8 @@ uint64_t align256(uint64_t x) { return (x + 255) & ~(uint64_t)255; }
 struct Layout {
   bool sorted = false, single = false;
   uint32_t tokens = 0, columns = 0, parts = 0, width = 0;
-  uint64_t delta = 0, head = 0, groups = 0, tile_first = 0, tile_groups = 0, req_col = 0, col_token = 0, hidden = 0, u = 0, end = 0;
+  uint64_t delta = 0, head = 0, groups = 0, tile_first = 0, tile_groups = 0, req_col = 0, col_token = 0, hidden = 0, u = 0, wide = 0,
+           end = 0;
 };
 
 Layout layout_of(const ft_adapter_args &a) {
@@ -856,14 +938,16 @@ Layout layout_of(const ft_adapter_args &a) {
   l.columns = (uint32_t)most;
   l.width = a.rank <= 16 ? 16 : a.rank <= 32 ? 32 : 64;
   l.parts = a.dtype == FT_DTYPE_BF16 && a.out_dtype == FT_DTYPE_F32 ? 3 : 2;
-  uint64_t at = l.single ? 0 : 256;
+  uint64_t at = 256;
   auto place = [&](uint64_t bytes) {
     const uint64_t here = at;
     at += align256(bytes);
     return here;
   };
+  l.u = place((uint64_t)((a.rank + l.width - 1) / l.width) * most * l.parts * l.width * 2);
+  l.col_token = place(4 * most);
+  l.wide = place(4ull * l.tokens * a.rank);
   if (l.single) {
-    l.u = place((uint64_t)((a.rank + l.width - 1) / l.width) * most * l.parts * l.width * 2);
     l.end = at;
     return l;
   }
@@ -871,9 +955,7 @@ Layout layout_of(const ft_adapter_args &a) {
   l.tile_first = place(4 * (most / 16 + 1));
   l.tile_groups = place(sizeof(Group) * kTileGroups * (most / plan_logits(a, l.columns, l.parts, l.width).tile_t + 1));
   l.req_col = place(4ull * a.n);
-  l.col_token = place(4 * most);
   l.hidden = place(most * a.dim * 2);
-  l.u = place((uint64_t)((a.rank + l.width - 1) / l.width) * most * l.parts * l.width * 2);
   l.end = at;
   return l;
 }
@@ -910,7 +992,7 @@ void adapter_logits_device(const ft_adapter_args &a, void *ws, uint64_t ws_bytes
     o = Sorted{reinterpret_cast<uint32_t *>(w + l.head),    reinterpret_cast<Group *>(w + l.groups),
                reinterpret_cast<uint32_t *>(w + l.tile_first),
                reinterpret_cast<Group *>(w + l.tile_groups), reinterpret_cast<uint32_t *>(w + l.req_col),
-               reinterpret_cast<int32_t *>(w + l.col_token), w + l.hidden,
+               reinterpret_cast<int32_t *>(w + l.col_token), reinterpret_cast<float *>(w + l.wide), w + l.hidden,
                w + l.u, l.columns, l.parts, l.width, l.single};
   const bool bf16 = a.dtype == FT_DTYPE_BF16;
   const CUtensorMap map_w = make_map(a.weight, bf16, a.dim, a.vocab, 0, kTileD, p.halves * kTileV, "weight");

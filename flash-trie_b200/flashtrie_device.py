@@ -339,9 +339,12 @@ def adapter_logits(hidden, weight, adapter_ids=None, lora_a=None, lora_b=None, s
     that request's logits NaN.  Without adapter_ids there are no adapters.
     Infinities and NaN in an adapter reach its own requests only; where lora_b
     or the product with lora_a is infinite the logit is NaN or infinite.
-    Products are summed in 32 bits and rounded once.  Returns [n, L, V] of
-    out_dtype (hidden's type, the default, or float32).  For serving: it has
-    no gradient."""
+    Products are summed in 32 bits and the logits rounded once; the low-rank
+    values between the two products may have any size that float32 holds and
+    lose 2^-17 at most (2^-26 for float32 logits of bfloat16 operands; float16
+    ones 2^-23, or 2^-25 absolute and 2^-17 of the token's largest).  Returns
+    [n, L, V] of out_dtype (hidden's type, the default, or float32).  For
+    serving: it has no gradient."""
     _want_floating(hidden, "hidden", 3, None, (torch.bfloat16, torch.float16))
     dev, dt = hidden.device, hidden.dtype
     _want(weight, "weight", dt, 2, dev)

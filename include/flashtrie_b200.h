@@ -241,9 +241,10 @@ int ft_tbs_batch_device_noalloc(ft_trie *trie, const ft_device_batch *batch,
  * outside [0, num_adapters) makes the request's logits NaN.  hidden, weight,
  * lora_a and lora_b are dtype (bf16 or f16), out is out_dtype (the same type,
  * or f32); all five start on 16-byte boundaries.  dim and rank are multiples
- * of 8, rank at most 256.  With f16 operands scale * (hidden lora_a) must stay
- * within f16's range (65504); 2^-23 of it is lost, or 2^-25 absolute.  An
- * infinite one, or an infinity in lora_b, makes the logits that it enters NaN
+ * of 8, rank at most 256.  scale * (hidden lora_a) may have any size that f32
+ * holds; 2^-17 of it is lost at most (2^-26 with bf16 operands and f32 logits),
+ * with f16 operands 2^-23, or 2^-25 absolute and 2^-17 of the token's largest.
+ * An infinite one, or an infinity in lora_b, makes the logits that it enters NaN
  * or infinite.  out overlaps none of the inputs.  num_adapters = 0: adapter_ids, lora_a, lora_b and
  * scale are not read.  scale may be NULL (1 for every adapter).  At most
  * 65536 adapters.
