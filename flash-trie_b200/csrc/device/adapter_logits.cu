@@ -760,10 +760,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t wrong = sh.wrong[n & 1][c0 / 32] >> (c0 % 32) & 0xFFFF;
         if (!kSorted && delta) {
           const uint32_t any = sh.more[n & 1][c0 / 32] >> (c0 % 32) & 0xFFFF;
+          // Not through the read-only path: this kernel may begin while the
+          // one before it still writes these.
           float add[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            add[e] = live && (any >> e & 1) ? __ldg(&delta[(uint64_t)(t0 + c0 + e) * vocab + v]) : 0.0f;
+            add[e] = live && (any >> e & 1) ? __ldcg(&delta[(uint64_t)(t0 + c0 + e) * vocab + v]) : 0.0f;
 #pragma unroll
           for (int e = 0; e < 16; ++e) acc[e] = __float_as_uint(__uint_as_float(acc[e]) + add[e]);
         }
