@@ -407,7 +407,7 @@ struct LogitsPlan {
 };
 
 struct alignas(16) LogitsShared {
-  uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
+  uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2], drained;
   // By turns for every other tile: where a column's logits begin in the output
   // (in bytes; negative: it has none), and which columns' logits are NaN.
   int64_t begin[2][kMaxTileT];
@@ -527,6 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     sh.gave_up = 0;
     for (uint32_t s = 0; s < p.stages; ++s) mbar_init(&sh.full[s], 1), mbar_init(&sh.empty[s], 1);
     for (int b = 0; b < 2; ++b) mbar_init(&sh.acc_full[b], 1), mbar_init(&sh.acc_empty[b], kEpilogue);
+    mbar_init(&sh.drained, 1);
     mbar_init_fence();
     prefetch_map(&map_w);
     prefetch_map(&map_h);
@@ -559,8 +560,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
 
   const bool lead = elect_one();
+  uint32_t sent = 0;  // stages filled so far (the loads' warp)
   if (warp == kLoadWarp) {
-    uint32_t at = 0, sent = 0;  // stage, and number of stages filled so far
+    uint32_t at = 0;  // stage
     bool ok = true;
     const uint8_t *low = o.u;
     const uint32_t slice = o.columns;
@@ -605,13 +607,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             next();
           });
     }
-    // Copies must not land in a block that has ended: wait for the last fill
-    // of each stage (the products saw all of them full if nothing failed).
-    if (!ok)
-      for (uint32_t s = 0; s < p.stages && s < sent; ++s) {
-        const uint32_t fill = (sent - 1 - s) / p.stages;
-        mbar_settle(&sh.full[s], fill & 1);
-      }
   } else if (warp == kProductWarp) {
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     uint32_t at = 0, phase = 0, n = 0;
@@ -821,6 +816,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   __syncwarp();
+  __syncthreads();
+  if (sh.gave_up) {
+    // Whichever warp gave up, neither copies nor products may be under way when
+    // the block ends: wait for the last fill of each stage, and for the products
+    // issued so far (if nothing failed the epilogue has seen all of them).
+    if (warp == kLoadWarp)
+      for (uint32_t s = 0; s < p.stages && s < sent; ++s) mbar_settle(&sh.full[s], (sent - 1 - s) / p.stages & 1);
+    if (warp == kProductWarp) {
+      mma_commit(&sh.drained, lead);
+      mbar_settle(&sh.drained, 0);
+    }
+  }
   fence_before();
   __syncthreads();
   fence_after();
