@@ -289,6 +289,15 @@ int ft_trie_device_status(ft_trie *trie, uint32_t *status) {
   });
 }
 
+int ft_trie_status_word(ft_trie *trie, uint32_t **word) {
+  return guarded([&] {
+    require_trie(trie);
+    if (!word) ftb::fail(ftb::ErrorKind::kNull, "MARISA_NULL_ERROR: word is NULL");
+    if (!trie->engine) ftb::fail(ftb::ErrorKind::kState, "MARISA_STATE_ERROR: no GPU workspace");
+    *word = trie->engine->status_word();
+  });
+}
+
 int ft_adapter_logits_workspace(const ft_adapter_args *args, uint64_t *bytes) {
   return guarded([&] {
     require_args(args, bytes);
@@ -297,9 +306,14 @@ int ft_adapter_logits_workspace(const ft_adapter_args *args, uint64_t *bytes) {
 }
 
 int ft_adapter_logits_device(const ft_adapter_args *args, void *workspace, uint64_t workspace_bytes, void *stream) {
+  return ft_adapter_logits_checked_device(args, nullptr, workspace, workspace_bytes, stream);
+}
+
+int ft_adapter_logits_checked_device(const ft_adapter_args *args, uint32_t *status, void *workspace,
+                                     uint64_t workspace_bytes, void *stream) {
   return guarded([&] {
     require_args(args);
-    ftb::adapter_logits_device(*args, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+    ftb::adapter_logits_device(*args, status, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
   });
 }
 

@@ -31,6 +31,7 @@
 #include "head_ops.hpp"
 #include "row_stream.cuh"
 #include "sm100.cuh"
+#include "tbs_kernel.cuh"
 
 namespace ftb {
 namespace {
@@ -515,7 +516,8 @@ template <typename T, typename O, bool kSorted>
 __global__ void __launch_bounds__(kThreads, 1)
     logits_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_h,
                   const __grid_constant__ CUtensorMap map_b, const __grid_constant__ ft_adapter_args a,
-                  const __grid_constant__ LogitsPlan p, const float *delta, const __grid_constant__ Sorted o) {
+                  const __grid_constant__ LogitsPlan p, const float *delta, const __grid_constant__ Sorted o,
+                  uint32_t *status) {
   using namespace sm100;
   extern __shared__ uint8_t raw[];
   uint8_t *buf = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
@@ -827,6 +829,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mma_commit(&sh.drained, lead);
       mbar_settle(&sh.drained, 0);
     }
+    if (threadIdx.x == 0 && status) atomicOr(status, kStatusLogits);
   }
   fence_before();
   __syncthreads();
@@ -976,9 +979,12 @@ uint64_t adapter_logits_workspace(const ft_adapter_args &a) {
   return layout_of(a).end;
 }
 
-void adapter_logits_device(const ft_adapter_args &a, void *ws, uint64_t ws_bytes, cudaStream_t stream) {
+void adapter_logits_device(const ft_adapter_args &a, uint32_t *status, void *ws, uint64_t ws_bytes,
+                           cudaStream_t stream) {
   check_adapter(a);
   if (a.n == 0) return;
+  if (reinterpret_cast<uintptr_t>(status) & 3)
+    throw InvalidArgument("adapter_logits: the status word is not aligned to its 4 bytes");
   const void *need[] = {a.hidden, a.weight, a.out};
   for (const void *p : need)
     if (!p) fail(ErrorKind::kNull, "MARISA_NULL_ERROR: adapter_logits: hidden, weight or out is NULL");
@@ -1022,7 +1028,8 @@ void adapter_logits_device(const ft_adapter_args &a, void *ws, uint64_t ws_bytes
   }
   auto logits = [&](auto *kernel) {
     allow_shared(kernel, 221 * 1024);
-    launch(a.num_adapters != 0, grid, kThreads, smem, stream, kernel, map_w, map_h, map_b, a, p, (const float *)delta, o);
+    launch(a.num_adapters != 0, grid, kThreads, smem, stream, kernel, map_w, map_h, map_b, a, p, (const float *)delta, o,
+           status);
   };
   auto run = [&](auto *t) {
     using T = std::remove_pointer_t<decltype(t)>;

@@ -25,6 +25,7 @@ void preference_loss_device(const ft_sequence_args &a, const ft_preference_args 
                             cudaStream_t stream);
 
 uint64_t adapter_logits_workspace(const ft_adapter_args &a);
-void adapter_logits_device(const ft_adapter_args &a, void *ws, uint64_t ws_bytes, cudaStream_t stream);
+void adapter_logits_device(const ft_adapter_args &a, uint32_t *status, void *ws, uint64_t ws_bytes,
+                           cudaStream_t stream);
 
 }  // namespace ftb

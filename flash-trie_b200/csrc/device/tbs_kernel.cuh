@@ -203,6 +203,7 @@ constexpr uint32_t kStatusNodeBounds = 8u;
 constexpr uint32_t kStatusBadRequest = 16u;
 constexpr uint32_t kStatusSelection = 32u;  // a selection did not select exactly k
 constexpr uint32_t kStatusHelp = 64u;       // a bounded wait on helper clusters ran out
+constexpr uint32_t kStatusLogits = 128u;    // a bounded wait of the vocabulary projection ran out
 
 // Shared-memory bytes the search kernel needs for a given max K / max final beam.
 size_t search_smem_bytes(uint32_t max_topk, uint32_t max_final_beam);

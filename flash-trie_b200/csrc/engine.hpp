@@ -58,6 +58,8 @@ class Engine {
   void search_host(const ft_request *reqs, uint32_t n, const ft_search_params &prm, ft_result *out);
   void search_device(const ft_device_batch &b, const ft_search_params &prm, cudaStream_t stream);
   uint32_t read_status();
+  // The device word that read_status() reads.
+  uint32_t *status_word() const { return d_status_dev_; }
   // Key ids of n token sequences in device memory, on `stream` (bad offsets
   // and trie inconsistencies go to the same status word as search_device).
   void lookup_device(uint32_t n, const uint32_t *tokens, const uint64_t *offsets, uint64_t total_tokens,

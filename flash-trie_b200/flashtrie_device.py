@@ -104,6 +104,8 @@ def _lib():
         lib.ft_reverse_lookup_batch_device.restype = ctypes.c_int
         lib.ft_trie_device_status.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_uint32)]
         lib.ft_trie_device_status.restype = ctypes.c_int
+        lib.ft_trie_status_word.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_void_p)]
+        lib.ft_trie_status_word.restype = ctypes.c_int
         lib.ft_last_error.restype = ctypes.c_char_p
         u64p, vp, u64 = ctypes.POINTER(ctypes.c_uint64), ctypes.c_void_p, ctypes.c_uint64
         for name, args in (("adapter_logits", _AdapterArgs), ("propose", _ProposeArgs),
@@ -111,6 +113,7 @@ def _lib():
             size, call = getattr(lib, "ft_%s_workspace" % name), getattr(lib, "ft_%s_device" % name)
             size.argtypes = [ctypes.POINTER(args), u64p]
             call.argtypes = [ctypes.POINTER(args), vp, u64, vp]
+        lib.ft_adapter_logits_checked_device.argtypes = [ctypes.POINTER(_AdapterArgs), vp, vp, u64, vp]
         lib.ft_sequence_grad_device.argtypes = [ctypes.POINTER(_SequenceArgs), vp, vp, vp, vp, u64, vp]
         lib.ft_preference_loss_workspace.argtypes = [ctypes.POINTER(_SequenceArgs), u64p]
         lib.ft_preference_loss_device.argtypes = [ctypes.POINTER(_SequenceArgs), ctypes.POINTER(_PreferenceArgs), vp,
@@ -325,7 +328,8 @@ class _On:
             c.__exit__(*error)
 
 
-def adapter_logits(hidden, weight, adapter_ids=None, lora_a=None, lora_b=None, scale=None, out_dtype=None, stream=None):
+def adapter_logits(hidden, weight, adapter_ids=None, lora_a=None, lora_b=None, scale=None, out_dtype=None, stream=None,
+                   status=None):
     """Logits of n requests over the vocabulary, each request with a low-rank
     adapter of its own beside the shared projection (C ABI
     ft_adapter_logits_device):
@@ -344,7 +348,21 @@ def adapter_logits(hidden, weight, adapter_ids=None, lora_a=None, lora_b=None, s
     lose 2^-17 at most (2^-26 for float32 logits of bfloat16 operands; float16
     ones 2^-23, or 2^-25 absolute and 2^-17 of the token's largest).  Returns
     [n, L, V] of out_dtype (hidden's type, the default, or float32).  For
-    serving: it has no gradient."""
+    serving: it has no gradient.
+
+    status: an int32 CUDA tensor of one element (or None).  The kernel's waits
+    are bounded; where one runs out it sets a bit there and leaves NaN in the
+    logits that it has not made.  Nothing clears the bit."""
+    if status is not None:
+        _want(status, "status", torch.int32, 1, hidden.device if isinstance(hidden, torch.Tensor) else None)
+        if status.numel() != 1:
+            raise ValueError("status must have one element")
+        status = status.data_ptr()
+    return _logits(hidden, weight, adapter_ids, lora_a, lora_b, scale, out_dtype, stream, status)
+
+
+def _logits(hidden, weight, adapter_ids, lora_a, lora_b, scale, out_dtype, stream, status):
+    """adapter_logits with the status word's address."""
     _want_floating(hidden, "hidden", 3, None, (torch.bfloat16, torch.float16))
     dev, dt = hidden.device, hidden.dtype
     _want(weight, "weight", dt, 2, dev)
@@ -382,7 +400,7 @@ def adapter_logits(hidden, weight, adapter_ids=None, lora_a=None, lora_b=None, s
         a = _AdapterArgs(*shape, hidden.data_ptr(), weight.data_ptr(), adapter_ids.data_ptr() if G else None,
                          lora_a.data_ptr() if G else None, lora_b.data_ptr() if G else None,
                          scale.data_ptr() if scale is not None else None, out.data_ptr())
-        _check(_lib().ft_adapter_logits_device(ctypes.byref(a), ws_ptr, ws_bytes, _raw_stream(dev)))
+        _check(_lib().ft_adapter_logits_checked_device(ctypes.byref(a), status, ws_ptr, ws_bytes, _raw_stream(dev)))
     return out
 
 
@@ -427,12 +445,17 @@ def bs_tbs_hidden(trie, beams, hidden, weight, k, token_logp_threshold, sents_lo
     """bs_tbs_device from a model's hidden states: adapter_logits (in
     logits_dtype), the k best proposals of each position, and the search, one
     after the other on `stream`.  hidden [n, L, D] goes with beams [n, L];
-    the other arguments and the outputs are those of the three calls."""
+    the other arguments and the outputs are those of the three calls.  A wait
+    of the projection that ran out is reported as the search's failures are:
+    raised with check=True, by device_status() otherwise."""
     _want(beams, "beams", torch.int32, 2, None)
     _want_floating(hidden, "hidden", 3, beams.device, (torch.bfloat16, torch.float16))
     if hidden.shape[:2] != beams.shape:
         raise ValueError("hidden must be [n, L, D] with n, L matching beams")
-    logits = adapter_logits(hidden, weight, adapter_ids, lora_a, lora_b, scale, out_dtype=logits_dtype, stream=stream)
+    word = ctypes.c_void_p()
+    if beams.shape[0]:
+        _check(_lib().ft_trie_status_word(ctypes.c_void_p(trie.ft_handle()), ctypes.byref(word)))
+    logits = _logits(hidden, weight, adapter_ids, lora_a, lora_b, scale, logits_dtype, stream, word)
     topk_id, topk_logp = propose(logits, k, stream=stream)
     del logits
     return bs_tbs_device(trie, beams, topk_id, topk_logp, token_logp_threshold, sents_logp_threshold, length_norm,

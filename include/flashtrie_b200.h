@@ -196,6 +196,10 @@ int ft_reverse_lookup_batch_device(ft_trie *trie, uint32_t n, const uint32_t *id
  * (0 = clean; the word is cleared by reading it); non-zero bits name the
  * checks that failed inside the kernel. */
 int ft_trie_device_status(ft_trie *trie, uint32_t *status);
+/* The device address of that word, for calls on the same device that report
+ * into it (ft_adapter_logits_checked_device).  It is the trie's until its GPU
+ * workspace is made anew or the trie destroyed. */
+int ft_trie_status_word(ft_trie *trie, uint32_t **word);
 
 /*
  * No counterpart in the reference.  The same search as ft_tbs_batch_device,
@@ -269,6 +273,11 @@ typedef struct {
 
 int ft_adapter_logits_workspace(const ft_adapter_args *args, uint64_t *bytes);
 int ft_adapter_logits_device(const ft_adapter_args *args, void *workspace, uint64_t workspace_bytes, void *stream);
+/* The same with a status word in device memory (or NULL): the kernel's waits
+ * are bounded, and where one runs out it sets a bit of *status and leaves NaN in
+ * the logits that it has not made.  Nothing clears the word. */
+int ft_adapter_logits_checked_device(const ft_adapter_args *args, uint32_t *status, void *workspace,
+                                     uint64_t workspace_bytes, void *stream);
 
 /*
  * The search's proposals from logits: per row, log-softmax over the
