@@ -364,7 +364,6 @@ __global__ void __launch_bounds__(kThreads, 2)
   const bool sampled = vocab > p.cap;
   const float bound = sampled ? sample_bound(sh, r, k) : kNegInf;
   __syncthreads();
-  SoftSum s = SoftSum::none();
   auto note = [&](int64_t i, float top) {
     if (top > bound) {
       const uint32_t at = atomicAdd(&sh.hits, 1u);
@@ -375,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   // are 3% slower, five no faster on bf16, and eight that are added up as soon
   // as they are all there 7%: the CTAs of a row that fits on the GPU at once
   // start together, and between the steps nothing would be on its way.
-  soft_stream<T, kThreads, 4>(r, v0, v1, bound, s, note);
+  SoftSum s = soft_stream<T, kThreads, 4>(r, v0, v1, bound, note);
   s = soft_join_block<kThreads>(s, sh.sums);  // a barrier: all hits are noted
   const uint32_t hits = sh.hits;
   if (hits <= p.hits)
@@ -426,11 +425,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (threadIdx.x < 32) {
       for (uint32_t c = threadIdx.x; c < p.chunks; c += 32)
         s = soft_join(s, SoftSum{__ldcg(&part[first + c].m), __ldcg(&part[first + c].z)});
-#pragma unroll
-      for (int d = 16; d; d >>= 1) {
-        const SoftSum o{__shfl_xor_sync(~0u, s.m, d), __shfl_xor_sync(~0u, s.z, d)};
-        s = soft_join(s, o);
-      }
+      s = soft_join_warp(s);
     }
     __syncthreads();
     uint32_t *before = sh.hist + 64;  // entries of the stretches before each

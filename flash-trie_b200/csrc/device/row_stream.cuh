@@ -24,11 +24,32 @@ __device__ __forceinline__ void from_f32(float v, float &o) { o = v; }
 __device__ __forceinline__ void from_f32(float v, __nv_bfloat16 &o) { o = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void from_f32(float v, __half &o) { o = __float2half_rn(v); }
 
-// e^d; d is a difference to a maximum, at most a rounding above 0.
+// e^d; d is a difference to a maximum or to a base a little below it.
 __device__ __forceinline__ float exp_below(float d) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaf(d, kLog2eRest, d * kLog2e)));
   return y;
+}
+
+// e^d for d <= 0 (a rounding above at most), for the few factors that whole sums
+// are multiplied by: the base-2 instruction's results are 5e-8 low on average,
+// which would add up from join to join.  Cody and Waite's reduction by multiples
+// of ln 2 in two parts, and Taylor's polynomial on [-ln 2 / 2, ln 2 / 2], whose
+// remainder is 5e-9 of the result; a step off at most in all.  0 below e^-86.
+__device__ __forceinline__ float exp_factor(float d) {
+  constexpr double kLn2 = 0.69314718055994530942;
+  constexpr float kHigh = (float)kLn2, kRest = (float)(kLn2 - (double)kHigh);
+  if (!(d > -86.0f)) return d != d ? d : 0.0f;
+  const float n = rintf(d * kLog2e), g = fmaf(-n, kRest, fmaf(-n, kHigh, d));
+  float p = 1.0f / 5040.0f;
+  p = fmaf(p, g, 1.0f / 720.0f);
+  p = fmaf(p, g, 1.0f / 120.0f);
+  p = fmaf(p, g, 1.0f / 24.0f);
+  p = fmaf(p, g, 1.0f / 6.0f);
+  p = fmaf(p, g, 0.5f);
+  p = fmaf(p, g, 1.0f);
+  p = fmaf(p, g, 1.0f);
+  return p * __int_as_float(((int)n + 127) << 23);
 }
 
 // A row's elements lie in 16-byte vectors counted from the aligned address at
@@ -130,29 +151,46 @@ __device__ __forceinline__ float top_of(uint4 q, const __half *) {
   return fmaxf(f.x, f.y);
 }
 
-// Running (maximum, sum of exp(x - maximum)).  A NaN or +inf among the values
-// leaves the sum NaN; nothing but -inf leaves (-inf, 0).
+// (maximum, sum of exp(x - maximum)).  A NaN or +inf among the values leaves the
+// sum NaN; nothing but -inf leaves (-inf, 0).  Exponentials are off by 2^-22 at
+// most, that of a difference of 0 is exact.
 struct SoftSum {
   float m, z;
   __device__ static SoftSum none() { return {kNegInf, 0.0f}; }
   __device__ bool valid() const { return z > 0.0f && z < -kNegInf; }  // false for NaN too
 };
 
-__device__ __forceinline__ float exp_from(float x, float m) {
-  return exp_below(x - (m == kNegInf ? 0.0f : m));
+// What a sum with maximum x is multiplied by under the maximum m >= x.
+__device__ __forceinline__ float factor_from(float x, float m) {
+  return exp_factor(x - (m == kNegInf ? 0.0f : m));
 }
+
+// A thread's sum under way, relative to a base that stays while the values pass
+// it by no more than kSlack (e^8 of room, of e^88): a base that followed every
+// new maximum would have the sum multiplied, and rounded, in most steps.
+struct SoftRun {
+  static constexpr float kSlack = 8.0f;
+  float m, base, z;  // largest value so far, base <= m, sum of exp(x - base)
+  __device__ static SoftRun none() { return {kNegInf, kNegInf, 0.0f}; }
+  __device__ __forceinline__ void raise(float top) {  // before values up to `top` are added
+    m = fmaxf(m, top);
+    if (top - base > kSlack) {  // hardly ever more than once after the first values
+      z *= exp_below(base - top);
+      base = top;
+    }
+  }
+  __device__ __forceinline__ float from() const { return base == kNegInf ? 0.0f : base; }
+  __device__ SoftSum sum() const { return {m, z * factor_from(base, m)}; }
+};
 
 // Returns the largest of the values (NaN ones aside).
 template <int N>
-__device__ __forceinline__ float soft_add(SoftSum &s, const float (&v)[N]) {
+__device__ __forceinline__ float soft_add(SoftRun &s, const float (&v)[N]) {
   float top = v[0];
 #pragma unroll
   for (int e = 1; e < N; ++e) top = fmaxf(top, v[e]);
-  if (top > s.m) {
-    s.z *= exp_from(s.m, top);
-    s.m = top;
-  }
-  const float base = s.m == kNegInf ? 0.0f : s.m;
+  s.raise(top);
+  const float base = s.from();
   float a = 0.0f;
 #pragma unroll
   for (int e = 0; e < N; ++e) a += exp_below(v[e] - base);
@@ -163,18 +201,15 @@ __device__ __forceinline__ float soft_add(SoftSum &s, const float (&v)[N]) {
 // The same for U whole vectors (and each one's largest value): one look at the
 // maximum for all of them.
 template <typename T, int U>
-__device__ __forceinline__ float soft_add(SoftSum &s, const uint4 (&q)[U], float (&tops)[U]) {
+__device__ __forceinline__ float soft_add(SoftRun &s, const uint4 (&q)[U], float (&tops)[U]) {
   constexpr int N = RowVecs<T>::N;
 #pragma unroll
   for (int u = 0; u < U; ++u) tops[u] = top_of(q[u], (const T *)nullptr);
   float top = tops[0];
 #pragma unroll
   for (int u = 1; u < U; ++u) top = fmaxf(top, tops[u]);
-  if (top > s.m) {
-    s.z *= exp_from(s.m, top);
-    s.m = top;
-  }
-  const float base = s.m == kNegInf ? 0.0f : s.m;
+  s.raise(top);
+  const float base = s.from();
   const float2 minus = make_float2(-base, -base);
   float2 a = make_float2(0.0f, 0.0f);
 #pragma unroll
@@ -191,32 +226,43 @@ __device__ __forceinline__ float soft_add(SoftSum &s, const uint4 (&q)[U], float
 __device__ __forceinline__ SoftSum soft_join(SoftSum a, SoftSum b) {
   SoftSum r;
   r.m = fmaxf(a.m, b.m);
-  r.z = a.z * exp_from(a.m, r.m) + b.z * exp_from(b.m, r.m);
+  r.z = a.z * factor_from(a.m, r.m) + b.z * factor_from(b.m, r.m);
   return r;
+}
+
+// Joins the sums of a warp in a fixed order: all lanes have the result.  The
+// maximum comes first, so that each sum is multiplied once.
+__device__ __forceinline__ SoftSum soft_join_warp(SoftSum s) {
+  float m = s.m;
+#pragma unroll
+  for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
+  s.z *= factor_from(s.m, m);
+  s.m = m;
+#pragma unroll
+  for (int d = 16; d; d >>= 1) s.z += __shfl_xor_sync(~0u, s.z, d);
+  return s;
 }
 
 // Joins the block's partial sums in a fixed order; thread 0 has the result.
 template <int THREADS>
 __device__ SoftSum soft_join_block(SoftSum s, SoftSum *smem /* [THREADS / 32] */) {
-#pragma unroll
-  for (int d = 16; d; d >>= 1) {
-    SoftSum o{__shfl_xor_sync(~0u, s.m, d), __shfl_xor_sync(~0u, s.z, d)};
-    s = soft_join(s, o);
-  }
+  constexpr int kWarps = THREADS / 32;
+  static_assert(kWarps <= 32, "a warp joins the warps' sums");
+  s = soft_join_warp(s);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = s;
   __syncthreads();
-  if (threadIdx.x == 0)
-    for (int w = 1; w < THREADS / 32; ++w) s = soft_join(s, smem[w]);
+  if (threadIdx.x < 32) s = soft_join_warp(threadIdx.x < kWarps ? smem[threadIdx.x] : SoftSum::none());
   return s;
 }
 
-// Adds the vectors [v0, v1) of a row to this thread's sum, U of them while U more
-// are on their way, and calls note(vector, its largest value) for those that may
-// hold something above `bound`.
+// This thread's share of the sum of a row's vectors [v0, v1), U of them added while
+// U more are on their way; calls note(vector, its largest value) for those that
+// may hold something above `bound`.
 template <typename T, int THREADS, int U, typename Note>
-__device__ __forceinline__ void soft_stream(const RowVecs<T> &r, int64_t v0, int64_t v1, float bound, SoftSum &s, Note &&note) {
+__device__ __forceinline__ SoftSum soft_stream(const RowVecs<T> &r, int64_t v0, int64_t v1, float bound, Note &&note) {
   constexpr int N = RowVecs<T>::N;
+  SoftRun s = SoftRun::none();
   constexpr int64_t kStep = U * THREADS;
   // The vectors that the row's ends cut, one by one; [w0, w1) are whole.
   const int64_t w0 = r.whole(v0) ? v0 : v0 + 1, w1 = v1 > w0 && !r.whole(v1 - 1) ? v1 - 1 : v1;
@@ -267,6 +313,7 @@ __device__ __forceinline__ void soft_stream(const RowVecs<T> &r, int64_t v0, int
     unpack(r.load_whole(i), v, (const T *)nullptr);
     note(i, soft_add(s, v));
   }
+  return s.sum();
 }
 
 }  // namespace ftb

@@ -1,8 +1,11 @@
 """How exact the model-side operators are, each property with data that leaves
-no room for anything else: weights of very different sizes,
-low-rank values far from 1.
+no room for anything else: sums whose terms are all 1, weights of very
+different sizes, low-rank values far from 1.
 
 Tolerances, derived here (U = 2^-24, half a step of f32):
+  - logits of 0 and -inf alone have exponentials of exactly 1 and 0, so that a
+    softmax sum is a count, exact in f32 up to 2^24 in any order; a 64-bit
+    logarithm is off by a step at most;
   - a weight of a preference pair is computed in 64 bits, rounded once as the
     candidate's gradient, once with the factors and once in the row: 3 U, and
     one more for the mean's factor; an upstream weight of a score is rounded
@@ -16,7 +19,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_head_ops import HALVES, U, gen, half_step, make_head
+from test_gpu_head_ops import HALVES, TYPES, U, gen, half_step, make_head
 
 pytestmark = pytest.mark.gpu
 
@@ -130,3 +133,75 @@ def test_low_rank_values_of_any_size(fd, t, n, L, G, scale, shared):
         assert bool((torch.isfinite(out) | beyond).all())
         err = torch.where(beyond, 0.0, (out - y).abs())
         assert bool((err <= tol).all()), float((err / (mass + shared_mass)).max())
+
+
+# ------------------------------------------------------------------- counts
+
+def counted(V, L, t, seed):
+    """Logits of 0 and -inf, the number of zeros of each row, and where one is."""
+    x = torch.zeros((1, L, V), device="cuda")
+    x[torch.rand((1, L, V), generator=gen(seed), device="cuda") < 0.3] = -math.inf
+    x[0, 0] = 0.0
+    live = torch.randint(0, V, (L,), generator=gen(seed + 1), device="cuda")
+    x[0, torch.arange(L), live] = 0.0
+    return x.to(t), (x == 0).sum(-1)[0].double(), live
+
+
+SIZES = [(1, 3), (5, 2), (777, 24), (4099, 24), (100003, 24), (100003, 2), (400009, 3), (2200000, 2)]
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("V,L", SIZES)
+def test_log_sums_count_every_value_once(fd, t, V, L):
+    """A value left out or taken twice anywhere in a row changes the count. The
+    margin shows the 64-bit score less its own rounding to f32."""
+    x, count, live = counted(V, L, t, seed=V)
+    want = -float(count.log().sum())
+    toks = live.to(torch.int32).view(1, 1, L).expand(1, 2, L).contiguous()
+    lens = torch.tensor([[L, 0]], dtype=torch.int32, device="cuda")
+    ref = torch.tensor([[want, 0.0]], device="cuda")
+    pair = [torch.tensor([[i]], dtype=torch.int32, device="cuda") for i in (0, 1)]
+    leaf = x.requires_grad_()
+    _, margin = fd.preference_loss(leaf, toks, lens, ref, *pair, beta=1.0)
+    rest = want - float(ref[0, 0].double())
+    assert abs(float(margin) - rest) <= L * 16 * 2.0 ** -52 + U * abs(rest)
+    lp = fd.sequence_logp(leaf, toks, lens)
+    assert abs(float(lp[0, 0].detach()) - want) <= U * abs(want) + L * 16 * 2.0 ** -52
+    # Every zero's gradient is -1 / count (the token's, 1 more): the division
+    # and the product are rounded, then the result.
+    (dx,) = torch.autograd.grad(lp[0, 0], leaf)
+    g = torch.where(x.detach() == 0, (-1 / count)[None, :, None], 0.0)
+    g[0, torch.arange(L), live] += 1.0
+    tol = 3 * U * g.abs() + half_step(t, g)
+    assert bool(((dx.double() - g).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("V,L", SIZES[:-1])
+def test_proposals_count_every_value_once(fd, t, V, L):
+    x, count, _ = counted(V, L, t, seed=V + 3)
+    _, lps = fd.propose(x, 1)
+    want = -count.log()
+    tol = 2 * U * want.abs()  # one step of the logarithm
+    assert V == 1 or bool((tol < 1 / count).all())
+    assert bool(((lps[0, :, 0].double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("V,R,seed", [(1001, 400, 1), (32000, 100, 2), (500009, 60, 3), (2200000, 24, 4)])
+def test_log_sums_do_not_lean(fd, t, V, R, seed):
+    """The mean error over many rows. The base-2 exponential is 5e-8 low on
+    average over its argument's fractions, and nothing that the joins do adds
+    to that; 3 / sqrt(R) of a sum's own spread (its terms' errors and a few dozen
+    roundings, 2 U) is left for the mean."""
+    x = torch.randn((R, 1, V), generator=gen(seed), device="cuda") * 2
+    x = (x - 0.3 * torch.log1p(torch.arange(V, device="cuda", dtype=torch.float32))).to(t)
+    top = x[:, 0].argmax(-1)
+    pair = [torch.full((R, 1), i, dtype=torch.int32, device="cuda") for i in (0, 1)]
+    toks = top.to(torch.int32).view(R, 1, 1).expand(R, 2, 1).contiguous()
+    lens = torch.tensor([1, 0], dtype=torch.int32, device="cuda").expand(R, 2).contiguous()
+    want = torch.stack([torch.log_softmax(x[i, 0].double(), -1)[top[i]] for i in range(R)])
+    ref = torch.stack([want.float(), torch.zeros(R, device="cuda")], 1).contiguous()
+    _, margin = fd.preference_loss(x, toks, lens, ref, *pair, beta=1.0)
+    off = margin[:, 0].double() - (want - ref[:, 0].double())
+    assert abs(float(off.mean())) <= 5e-8 + 3 / math.sqrt(R) * 2 * U, (float(off.mean()), float(off.std()))
