@@ -308,9 +308,11 @@ def _raw_stream(device):
 
 
 class _On:
-    """The call's device and stream made current, where they are not already."""
+    """The call's device and stream made current, where they are not already.
+    Inputs are noted as in use on a stream that is not the current one: their
+    memory, if the caller drops them, waits for what that stream has to do."""
 
-    def __init__(self, device, stream):
+    def __init__(self, device, stream, *inputs):
         self.inner = []
         if stream is not None and stream.device_index != device.index:
             raise ValueError("stream must be of the tensors' device, cuda:%d" % device.index)
@@ -318,6 +320,10 @@ class _On:
             self.inner.append(torch.cuda.device(device))
         if stream is not None:
             self.inner.append(torch.cuda.stream(stream))
+            if stream != torch.cuda.current_stream(device):
+                for t in inputs:
+                    if t is not None:
+                        t.record_stream(stream)
 
     def __enter__(self):
         for c in self.inner:
@@ -394,7 +400,7 @@ def _logits(hidden, weight, adapter_ids, lora_a, lora_b, scale, out_dtype, strea
     if L == 0 or V == 0 or D == 0:
         raise ValueError("L, V and D must be positive")
     shape = (n, L, V, D, r, G, _DTYPE[dt], _DTYPE[out_dtype])
-    with _On(dev, stream):
+    with _On(dev, stream, hidden, weight, adapter_ids, lora_a, lora_b, scale):
         ws, ws_ptr, ws_bytes = _workspace(dev, "ft_adapter_logits_workspace", _AdapterArgs, *shape)
         out = torch.empty(n, L, V, dtype=out_dtype, device=dev)
         a = _AdapterArgs(*shape, hidden.data_ptr(), weight.data_ptr(), adapter_ids.data_ptr() if G else None,
@@ -429,7 +435,7 @@ def propose(logits, k, order="id", stream=None):
         raise ValueError("the vocabulary is empty")
     _no_gradient("propose", logits=logits)
     shape = (n * L, V, k, _DTYPE[logits.dtype], int(order == "logp"))
-    with _On(dev, stream):
+    with _On(dev, stream, logits):
         ids = torch.empty(n, L, k, dtype=torch.int32, device=dev)
         lps = torch.empty(n, L, k, dtype=torch.float32, device=dev)
         if n * L:
@@ -458,6 +464,7 @@ def bs_tbs_hidden(trie, beams, hidden, weight, k, token_logp_threshold, sents_lo
     logits = _logits(hidden, weight, adapter_ids, lora_a, lora_b, scale, logits_dtype, stream, word)
     topk_id, topk_logp = propose(logits, k, stream=stream)
     del logits
+    _On(beams.device, stream, beams)
     return bs_tbs_device(trie, beams, topk_id, topk_logp, token_logp_threshold, sents_logp_threshold, length_norm,
                          early_exit, capacity=capacity, stream=stream, check=check, key_ids=key_ids)
 
@@ -582,7 +589,7 @@ def sequence_logp(logits, tokens, lengths, stream=None):
     all -inf, has log-probability -inf.  The gradient is deterministic; the
     backward pass runs on the forward call's stream."""
     dev = _want_candidates(logits, tokens, lengths)
-    with _On(dev, stream):
+    with _On(dev, stream, logits, tokens, lengths):
         if logits.requires_grad and torch.is_grad_enabled():
             return _SequenceLogp.apply(logits, tokens, lengths)
         return _scores(logits, tokens, lengths)[0]
@@ -624,7 +631,7 @@ def preference_loss(logits, tokens, lengths, ref_logp, chosen, rejected, beta=0.
     if reduction not in ("mean", "sum"):
         raise ValueError("reduction must be 'mean' or 'sum'")
     args = (logits, tokens, lengths, ref_logp, chosen, rejected, beta, label_smoothing, reduction == "mean")
-    with _On(dev, stream):
+    with _On(dev, stream, *args[:6]):
         if logits.requires_grad and torch.is_grad_enabled():
             return _PreferenceLoss.apply(*args)
         return _preference(*args)[:2]
