@@ -19,7 +19,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_head_ops import HALVES, TYPES, U, gen, half_step, make_head
+from test_gpu_head_ops import HALVES, TYPES, U, gen, half_step, make_head, make_logits, spread
 
 pytestmark = pytest.mark.gpu
 
@@ -135,6 +135,38 @@ def test_low_rank_values_of_any_size(fd, t, n, L, G, scale, shared):
         assert bool((err <= tol).all()), float((err / (mass + shared_mass)).max())
 
 
+@pytest.mark.parametrize("t", HALVES)
+@pytest.mark.parametrize("n,L,G", FORMS)
+def test_low_rank_parts_hold_what_they_say(fd, t, n, L, G):
+    """One product alone: h, A and B are single ones, so that the logit is the
+    adapter's scale, all of its 24 bits but what the parts lose."""
+    D, V, r = 64, 130, 16
+    h = torch.zeros((n, L, D), dtype=t, device="cuda")
+    h[..., 3] = 1.0
+    a = torch.zeros((G, r, D), dtype=t, device="cuda")
+    a[:, 5, 3] = 1.0
+    b = torch.zeros((G, V, r), dtype=t, device="cuda")
+    b[:, :, 5] = 1.0
+    s = torch.rand(G, generator=gen(4), device="cuda") + 0.5
+    ids = (torch.arange(n, device="cuda") % G).to(torch.int32)
+    out = fd.adapter_logits(h, torch.zeros((V, D), dtype=t, device="cuda"), ids, a, b, s, out_dtype=torch.float32)
+    want = s.double()[ids.long()][:, None, None]
+    assert bool(((out.double() - want).abs() <= LOSS[t, True] * want).all())
+
+
+def test_long_sums_are_two_of_half_the_length(fd):
+    """f32 logits, all products positive: a sum of 2048 is off by no more than
+    one of 1024 (as many partial sums are cut in each of its halves; a quarter
+    is left for the spread of the mean)."""
+    off = []
+    for D in (1024, 2048):
+        h = torch.randn((1, 16, D), generator=gen(5), device="cuda").abs().to(torch.bfloat16)
+        w = torch.randn((4096, D), generator=gen(6), device="cuda").abs().to(torch.bfloat16)
+        y = h.double() @ w.double().T
+        off.append(abs(float(((fd.adapter_logits(h, w, out_dtype=torch.float32).double() - y) / y).mean())))
+    assert off[1] <= 1.25 * off[0], off
+
+
 # ------------------------------------------------------------------- counts
 
 def counted(V, L, t, seed):
@@ -205,3 +237,22 @@ def test_log_sums_do_not_lean(fd, t, V, R, seed):
     _, margin = fd.preference_loss(x, toks, lens, ref, *pair, beta=1.0)
     off = margin[:, 0].double() - (want - ref[:, 0].double())
     assert abs(float(off.mean())) <= 5e-8 + 3 / math.sqrt(R) * 2 * U, (float(off.mean()), float(off.std()))
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("V,L", [(4099, 24), (100003, 24), (100003, 2), (300001, 3)])
+def test_log_sums_of_ordinary_rows(fd, t, V, L):
+    """A thread of 512 adds V / 512 values and a few more for the row's ends and
+    the joins; an exponential's argument is off by 2 U of the spread, the
+    exponential by 4 U."""
+    x = make_logits(1, L, V, t, seed=V + L, masked=False)
+    xd = x.double()
+    lp = torch.log_softmax(xd, -1)
+    top = xd.argmax(-1)
+    want = lp.gather(2, top[..., None])[0, :, 0]
+    tol = (4 * spread(xd)[0] + 8 + V / 512 + 112) * U + 2 * U * want.abs()
+    _, got = fd.propose(x, 1)
+    assert bool(((got[0, :, 0].double() - want).abs() <= tol).all())
+    toks = top.view(L, 1, 1).to(torch.int32)
+    score = fd.sequence_logp(x.view(L, 1, V), toks, torch.ones((L, 1), dtype=torch.int32, device="cuda"))
+    assert bool(((score[:, 0].double() - want).abs() <= tol).all())
