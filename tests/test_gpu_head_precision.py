@@ -43,7 +43,7 @@ def spiked(C):
 
 
 @pytest.mark.parametrize("lo,hi,P,absent", [(25, 40, 1000, 0), (36, 50, 200, 0), (36, 60, 200, 0),
-                                            (-5, 75, 1000, 0), (0, 40, 1, 0),
+                                            (-5, 75, 1000, 0), (0, 40, 1, 0), (-5, 60, 3001, 0), (10, 60, 8191, 1),
                                             (20, 30, 3, 200000)])
 @pytest.mark.parametrize("reduction", ["sum", "mean"])
 def test_pair_weights_of_any_margin(fd, lo, hi, P, absent, reduction):
@@ -111,13 +111,18 @@ def test_low_rank_values_of_any_size(fd, t, n, L, G, scale, shared):
     ids = (torch.arange(n, device="cuda") % G).to(torch.int32)
     if not shared:
         w = torch.zeros_like(w)
-    s = s * scale
-    at = ids.long()
+    check_low_rank(fd, h, w, ids, a, b, s * scale)
+
+
+def check_low_rank(fd, h, w, ids, a, b, s):
+    t, D, r = h.dtype, h.shape[2], a.shape[1]
+    at = ids.long().clamp(min=0)
     hd, ad, bd = h.double(), a.double()[at], b.double()[at]
-    u = (hd @ ad.transpose(1, 2)) * s.double()[at][:, None, None]
+    f = torch.where(ids >= 0, s.double()[at], 0.0)[:, None, None]
+    u = (hd @ ad.transpose(1, 2)) * f
     y = hd @ w.double().T + u @ bd.transpose(1, 2)
     shared_mass = hd.abs() @ w.double().abs().T
-    u_mass = (hd.abs() @ ad.abs().transpose(1, 2)) * s.double()[at][:, None, None] @ bd.abs().transpose(1, 2)
+    u_mass = (hd.abs() @ ad.abs().transpose(1, 2)) * f @ bd.abs().transpose(1, 2)
     mass = u.abs() @ bd.abs().transpose(1, 2)
     for out_t in (t, torch.float32):
         out = fd.adapter_logits(h, w, ids, a, b, s, out_dtype=out_t).double()
@@ -133,6 +138,22 @@ def test_low_rank_values_of_any_size(fd, t, n, L, G, scale, shared):
         assert bool((torch.isfinite(out) | beyond).all())
         err = torch.where(beyond, 0.0, (out - y).abs())
         assert bool((err <= tol).all()), float((err / (mass + shared_mass)).max())
+
+
+@pytest.mark.parametrize("t", HALVES)
+@pytest.mark.parametrize("n,L,V,D,r,G", [(1, 300, 8001, 72, 64, 1), (1, 7, 80000, 64, 16, 2), (20, 20, 76000, 136, 40, 6),
+                                         (2, 30, 76032, 1160, 72, 3), (9, 33, 777, 64, 256, 2), (64, 4, 515, 64, 32, 9)])
+def test_tokens_of_all_sizes_side_by_side(fd, t, n, L, V, D, r, G):
+    """Tokens whose low-rank values the 16-bit parts hold beside tokens whose
+    values they do not, in several tiles and slices, requests without an
+    adapter among them."""
+    h, w, ids, a, b, s = make_head(n, L, V, D, r, G, t, seed=11)
+    size = 2.0 ** (torch.randint(0, 3, (n, L, 1), generator=gen(12), device="cuda") * 12 - 12).double()
+    h = (h.double() * size).to(t)
+    b = (b.double() * 2.0 ** -6).to(t)
+    if n == 1:
+        ids = torch.zeros_like(ids)
+    check_low_rank(fd, h, w, ids, a, b, s * 2.0 ** 5)
 
 
 @pytest.mark.parametrize("t", HALVES)
