@@ -227,8 +227,8 @@ constexpr int kShrinkTokens = 4, kShrinkRows = 4;
 // the parts of eight columns next to one another; the values meet in shared
 // memory before, where each token's largest decides whether parts hold them.
 // Tokens four to a CTA, so that
-// a few of them spread over many SMs: latency, 2.7 us for 8 tokens of D = 512
-// and 5.8 for 128 of 768; 20 us for 1280 tokens of 2048 and rank 64, each CTA
+// a few of them spread over many SMs: latency, 3.6 us for 8 tokens of D = 512
+// and 6.5 for 128 of 768; 23 us for 1280 tokens of 2048 and rank 64, each CTA
 // reading its adapter's rows from L2.
 template <typename T, bool kSorted>
 __global__ void __launch_bounds__(256) shrink_kernel(ft_adapter_args a, float *u, Sorted o) {
@@ -345,8 +345,8 @@ constexpr int kExpandThreads = 256, kExpandRows = 4, kExpandTokens = 4;
 // The direct form's low-rank part: four vocabulary entries per thread, 256
 // apart, for the tokens of one request. What costs here is getting to the rows
 // of B, so that four are on their way at once; rows staged through shared
-// memory in whole lines came out three times slower. 7.3 us for 37 single
-// tokens with 40 adapters by 32000 of rank 16 (38 MB of rows, 5.2 TB/s).
+// memory in whole lines came out three times slower. 7.7 us for 37 single
+// tokens with 40 adapters by 32000 of rank 16 (38 MB of rows, 4.9 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(kExpandThreads) expand_kernel(ft_adapter_args a, const float *u, float *delta) {
   sm100::launch_next();
@@ -444,7 +444,9 @@ LogitsPlan plan_logits(const ft_adapter_args &a, uint32_t columns, uint32_t part
 }
 size_t logits_smem(const LogitsPlan &p) { return 1024 + (size_t)p.stages * p.stage; }
 
-// sum_r u[r] b[r] of a token whose low-rank values are in 32 bits alone.
+// sum_r u[r] b[r] of a token whose low-rank values are in 32 bits alone. Rows of B
+// come one by one: with such tokens alone, 0.64 ms instead of 0.17 for 20 tokens
+// by 500k x 1024 of rank 16, 8 instead of 0.55 for 1280 by 100k x 2048 of rank 64.
 template <typename T>
 __device__ __noinline__ float wide_part(const T *b, const float *u, uint32_t rank) {
   float s = 0.0f;
@@ -506,10 +508,10 @@ __device__ __forceinline__ bool walk_tile(const Walk &k, bool sorted, const Grou
 //
 // Few tokens: bound by the weight's bytes, 688 us for 20 tokens by 2.2M x 1024
 // bf16 (4.6 GB, 6.7 TB/s), 156 us for 128 by 500k x 768 with f32 logits (1.02
-// GB, 6.6 TB/s) and 179 with eight adapters.  Full batches: bound by what an SM
+// GB, 6.6 TB/s) and 182 with eight adapters.  Full batches: bound by what an SM
 // takes in and by the power limit.  1280 tokens by 500k x 2048 with 16 adapters
-// of rank 64 take 2.39 ms (1130 TFLOP/s of useful products).  By 100k, the shared
-// product alone takes 379 us (1384 TFLOP/s) and with adapters 470 to 490: the
+// of rank 64 take 2.39 to 2.5 ms (1080 to 1130 TFLOP/s of useful products).  By
+// 100k, the shared product alone takes 382 us (1373 TFLOP/s) and with adapters 485 to 500: the
 // padded columns make a sixth tile of tokens, which loads the weight once more
 // (a seventh of the time), the rest are the adapters' rows and values.
 template <typename T, typename O, bool kSorted>

@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(kStatThreads, 4)
 // Scores of 32 candidates of one request: eight lanes each, which take every
 // eighth position and add in 64 bits (a preference's margin is a small
 // difference of such sums). Latency of one look at the statistics and one at
-// each logit: 3 us for 10 candidates of 8 positions, 6.5 us for 1000 of 24.
+// each logit: 3 us for 10 candidates of 8 positions, 6.9 us for 1000 of 24.
 template <typename T>
 __global__ void __launch_bounds__(kScoreThreads)
     score_kernel(const T *logits, const uint32_t *tokens, const int32_t *lengths, uint32_t vocab, uint32_t L, uint32_t C,
@@ -176,8 +176,8 @@ __device__ __forceinline__ void add_shared(unsigned long long *sum, unsigned lon
 // each candidate's sum has a unit of its own, by its largest weight: the first
 // pass finds that and the second adds (a thread keeps its first pair's weight,
 // those of further pairs are worked out again).  The CTA that ends last adds up
-// the requests.  Latency of looks one after the other: 9.4 us for 1000 pairs,
-// 7.7 for 8.
+// the requests.  Latency of looks one after the other: 10.1 us for 1000 pairs,
+// 8.0 for 8.
 __global__ void __launch_bounds__(kPairThreads)
     pair_kernel(ft_preference_args p, uint32_t n, uint32_t C, const double *logp64, double2 *part, uint32_t *ticket) {
   // [C] sums, u32 [C] the power above each one's largest weight (0: no pair),
@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(kPairThreads)
 // list's order is not, and nothing depends on it.  Each token's sum has a unit
 // of its own, by the exponent of its largest weight, which the first pass finds.
 // A weight that is not finite makes W NaN, and with it the row's gradient.
-// Latency: 5.9 us for 48 rows of 1000 candidates, 4.1 for 128 of 10.
+// Latency: 6.2 us for 48 rows of 1000 candidates, 4.1 for 128 of 10.
 __global__ void __launch_bounds__(kPlanThreads)
     scatter_plan_kernel(const uint32_t *tokens, const int32_t *lengths, const SoftSum *stats, const float *grad,
                         const float *factor, const float *upstream, uint32_t vocab, uint32_t L, uint32_t C,

@@ -19,10 +19,10 @@
 // with a bound that rises (`careful`), and a row that kept fewer than k is read
 // again by its last CTA without one.
 //
-// Large batches are bound by the logits' bytes: 92 us for 256 rows of 500009 f32
-// (512 MB, 5.6 TB/s), k 256, a CTA per row.  One request is bound by latency
-// around its stream: 47.5 us for 20 rows of 2.2M bf16 (88 MB, 13.5 us at the
-// copy rate), k 1000; 14.5 us for 8 rows of 32000 f32, k 64.
+// Large batches are bound by the logits' bytes: 93 us for 256 rows of 500009 f32
+// (512 MB, 5.5 TB/s), k 256, a CTA per row.  One request is bound by latency
+// around its stream: 47.3 us for 20 rows of 2.2M bf16 (88 MB, 13.5 us at the
+// copy rate), k 1000; 14.7 us for 8 rows of 32000 f32, k 64.
 #include <algorithm>
 #include <string>
 
